@@ -680,6 +680,263 @@ void moe_router_fwd(py::handle logits, py::handle topk_weights, py::handle topk_
                                      lv.dtype, renormalize ? 1 : 0, st));
 }
 
+// As moe_permutation_fwd, with where each expert's entries begin.
+void moe_permutation_offsets_fwd(py::handle topk_indices, py::handle permute_index, py::handle unpermute_index,
+                                 py::handle expert_offsets, int64_t num_experts) {
+  View tv = validate_int64_tensor("topk_indices", topk_indices);
+  View pv = validate_int64_tensor("permute_index", permute_index);
+  View uv = validate_int64_tensor("unpermute_index", unpermute_index);
+  View ov = validate_int64_tensor("expert_offsets", expert_offsets);
+  if (tv.shape.size() != 2) {
+    shape_mismatch("topk_indices must be 2-D [num_tokens, k], got " + shape_str(tv.shape));
+  }
+  const int64_t n_tokens = tv.shape[0], k = tv.shape[1];
+  if (num_experts < 1 || num_experts > 256) {
+    shape_mismatch("num_experts (" + std::to_string(num_experts) + ") must be in [1, 256]");
+  }
+  if (pv.shape != std::vector<int64_t>{n_tokens * k}) {
+    shape_mismatch("permute_index shape " + shape_str(pv.shape) + " must be [" + std::to_string(n_tokens * k) + "]");
+  }
+  if (uv.shape != tv.shape) {
+    shape_mismatch("unpermute_index shape " + shape_str(uv.shape) + " must match topk_indices' " +
+                   shape_str(tv.shape));
+  }
+  if (ov.shape != std::vector<int64_t>{num_experts + 1}) {
+    shape_mismatch("expert_offsets shape " + shape_str(ov.shape) + " must be [" + std::to_string(num_experts + 1) +
+                   "] (num_experts + 1)");
+  }
+  const Launch launch(tv.device_index);
+  check_launch("launch_moe_permutation_offsets_fwd",
+               launch_moe_permutation_offsets_fwd((const int64_t*)tv.ptr, (int64_t*)pv.ptr, (int64_t*)uv.ptr,
+                                                  (int64_t*)ov.ptr, n_tokens, k, num_experts, launch.st));
+}
+
+// ---- expert products and MXFP4 (additive) -----------------------------------
+
+void check_same_device(const char* name, const View& v, const View& expected, const char* ref) {
+  if (v.device_index != expected.device_index) {
+    value_error(std::string("device mismatch: '") + name + "' is on cuda:" + std::to_string(v.device_index) +
+                " but '" + ref + "' is on cuda:" + std::to_string(expected.device_index));
+  }
+}
+
+void require_float(const char* name, const View& v) {
+  if (v.dtype != F32 && v.dtype != F16 && v.dtype != BF16) {
+    unsupported_dtype(std::string(name) + " is " + tag_debug(v.dtype));
+  }
+}
+
+constexpr int64_t kMaxExperts = 1024, kMaxRowBytes = int64_t(1) << 22;
+
+int64_t check_offsets(const View& offsets) {
+  if (offsets.shape.size() != 1 || offsets.shape[0] < 2 || offsets.shape[0] > kMaxExperts + 1) {
+    shape_mismatch("offsets must be 1-D [num_experts + 1] with num_experts in [1, " + std::to_string(kMaxExperts) +
+                   "], got " + shape_str(offsets.shape));
+  }
+  return offsets.shape[0] - 1;
+}
+
+// Limits of the launchers that no shape check covers.
+void check_product_sizes(int64_t rows, int64_t n_bytes, int64_t k_bytes) {
+  if (rows > INT32_MAX) shape_mismatch("more than 2^31 - 1 rows (" + std::to_string(rows) + ")");
+  if (n_bytes > kMaxRowBytes || k_bytes > kMaxRowBytes) {
+    shape_mismatch("rows of more than 4 MiB (" + std::to_string(n_bytes > k_bytes ? n_bytes : k_bytes) + " bytes)");
+  }
+}
+
+int64_t dtype_bytes(int32_t tag) { return tag == F32 ? 4 : 2; }
+
+void grouped_linear_fwd(py::handle x, py::handle weight, py::handle offsets, py::handle y) {
+  View xv = validate_tensor("x", x);
+  View wv = validate_tensor("weight", weight);
+  View ov = validate_int64_tensor("offsets", offsets);
+  View yv = validate_tensor("y", y);
+  require_float("x", xv);
+  check_dtype_matches("weight", wv, xv, "x");
+  check_dtype_matches("y", yv, xv, "x");
+  check_same_device("weight", wv, xv, "x");
+  check_same_device("offsets", ov, xv, "x");
+  check_same_device("y", yv, xv, "x");
+  if (xv.shape.size() != 2) shape_mismatch("x must be 2-D [rows, k], got " + shape_str(xv.shape));
+  const int64_t experts = check_offsets(ov);
+  if (wv.shape.size() != 3 || wv.shape[0] != experts || wv.shape[2] != xv.shape[1]) {
+    shape_mismatch("weight must be [num_experts, n, k] = [" + std::to_string(experts) + ", n, " +
+                   std::to_string(xv.shape[1]) + "], got " + shape_str(wv.shape));
+  }
+  const int64_t rows = xv.shape[0], k = xv.shape[1], n = wv.shape[1];
+  if (yv.shape != std::vector<int64_t>{rows, n}) {
+    shape_mismatch("y shape " + shape_str(yv.shape) + " must be [" + std::to_string(rows) + ", " + std::to_string(n) +
+                   "]");
+  }
+  check_product_sizes(rows, n * dtype_bytes(xv.dtype), k * dtype_bytes(xv.dtype));
+  const Launch launch(xv.device_index);
+  check_launch("launch_grouped_linear_fwd",
+               launch_grouped_linear_fwd((const void*)xv.ptr, (const void*)wv.ptr, (const int64_t*)ov.ptr,
+                                         (void*)yv.ptr, rows, experts, n, k, xv.dtype, launch.st));
+}
+
+void grouped_linear_grad_input(py::handle grad_y, py::handle weight, py::handle offsets, py::handle grad_x) {
+  View gv = validate_tensor("grad_y", grad_y);
+  View wv = validate_tensor("weight", weight);
+  View ov = validate_int64_tensor("offsets", offsets);
+  View xv = validate_tensor("grad_x", grad_x);
+  require_float("grad_y", gv);
+  check_dtype_matches("weight", wv, gv, "grad_y");
+  check_dtype_matches("grad_x", xv, gv, "grad_y");
+  check_same_device("weight", wv, gv, "grad_y");
+  check_same_device("offsets", ov, gv, "grad_y");
+  check_same_device("grad_x", xv, gv, "grad_y");
+  if (gv.shape.size() != 2) shape_mismatch("grad_y must be 2-D [rows, n], got " + shape_str(gv.shape));
+  const int64_t experts = check_offsets(ov);
+  if (wv.shape.size() != 3 || wv.shape[0] != experts || wv.shape[1] != gv.shape[1]) {
+    shape_mismatch("weight must be [num_experts, n, k] = [" + std::to_string(experts) + ", " +
+                   std::to_string(gv.shape[1]) + ", k], got " + shape_str(wv.shape));
+  }
+  const int64_t rows = gv.shape[0], n = gv.shape[1], k = wv.shape[2];
+  if (xv.shape != std::vector<int64_t>{rows, k}) {
+    shape_mismatch("grad_x shape " + shape_str(xv.shape) + " must be [" + std::to_string(rows) + ", " +
+                   std::to_string(k) + "]");
+  }
+  check_product_sizes(rows, n * dtype_bytes(gv.dtype), k * dtype_bytes(gv.dtype));
+  const Launch launch(gv.device_index);
+  check_launch("launch_grouped_linear_grad_input",
+               launch_grouped_linear_grad_input((const void*)gv.ptr, (const void*)wv.ptr, (const int64_t*)ov.ptr,
+                                                (void*)xv.ptr, rows, experts, n, k, gv.dtype, launch.st));
+}
+
+void grouped_linear_grad_weight(py::handle grad_y, py::handle x, py::handle offsets, py::handle grad_weight) {
+  View gv = validate_tensor("grad_y", grad_y);
+  View xv = validate_tensor("x", x);
+  View ov = validate_int64_tensor("offsets", offsets);
+  View wv = validate_tensor("grad_weight", grad_weight);
+  require_float("grad_y", gv);
+  check_dtype_matches("x", xv, gv, "grad_y");
+  check_dtype_matches("grad_weight", wv, gv, "grad_y");
+  check_same_device("x", xv, gv, "grad_y");
+  check_same_device("offsets", ov, gv, "grad_y");
+  check_same_device("grad_weight", wv, gv, "grad_y");
+  if (gv.shape.size() != 2 || xv.shape.size() != 2 || gv.shape[0] != xv.shape[0]) {
+    shape_mismatch("grad_y [rows, n] and x [rows, k] must be 2-D with the same rows; got grad_y=" +
+                   shape_str(gv.shape) + ", x=" + shape_str(xv.shape));
+  }
+  const int64_t experts = check_offsets(ov);
+  const int64_t rows = gv.shape[0], n = gv.shape[1], k = xv.shape[1];
+  if (wv.shape != std::vector<int64_t>{experts, n, k}) {
+    shape_mismatch("grad_weight shape " + shape_str(wv.shape) + " must be [" + std::to_string(experts) + ", " +
+                   std::to_string(n) + ", " + std::to_string(k) + "]");
+  }
+  check_product_sizes(rows, n * dtype_bytes(gv.dtype), k * dtype_bytes(gv.dtype));
+  const Launch launch(gv.device_index);
+  check_launch("launch_grouped_linear_grad_weight",
+               launch_grouped_linear_grad_weight((const void*)gv.ptr, (const void*)xv.ptr, (const int64_t*)ov.ptr,
+                                                 (void*)wv.ptr, rows, experts, n, k, gv.dtype, launch.st));
+}
+
+// Codes of MXFP4 (uint8) or its scales (float8_e8m0fnu).
+View validate_mxfp4(const char* name, const py::handle& obj, const char* dtype) {
+  RawView r = validate_and_extract(name, obj);
+  if (r.dtype_str != std::string("torch.") + dtype) {
+    value_error(std::string("unsupported dtype '") + r.dtype_str + "': " + name + " must be " + dtype);
+  }
+  return View{r.ptr, -1, r.device_index, std::move(r.shape)};
+}
+View validate_codes(const char* name, const py::handle& obj) { return validate_mxfp4(name, obj, "uint8"); }
+View validate_e8m0(const char* name, const py::handle& obj) { return validate_mxfp4(name, obj, "float8_e8m0fnu"); }
+
+// codes [..., 16 * blocks] and scales [..., blocks] of the same leading dimensions.
+void check_mxfp4_pair(const char* what, const View& codes, const View& scales) {
+  std::vector<int64_t> want = codes.shape;
+  const bool whole = !want.empty() && want.back() % 16 == 0;
+  if (whole) want.back() /= 16;
+  if (!whole || scales.shape != want) {
+    shape_mismatch(std::string(what) + " codes [..., 16 * blocks] and scales [..., blocks] do not belong together; got " +
+                   shape_str(codes.shape) + " and " + shape_str(scales.shape));
+  }
+}
+
+// rows x width of a tensor against its codes: [..., 16 * ceil(width / 32)].
+int64_t check_mxfp4_rows(const View& full, const char* name, const View& codes) {
+  std::vector<int64_t> want = full.shape;
+  if (want.empty()) shape_mismatch(std::string(name) + " must have at least 1 dimension");
+  const int64_t width = want.back();
+  want.back() = (width + 31) / 32 * 16;
+  if (codes.shape != want) {
+    shape_mismatch("codes shape " + shape_str(codes.shape) + " must be " + shape_str(want) + " for " + name + " " +
+                   shape_str(full.shape));
+  }
+  if (width > INT32_MAX) shape_mismatch("rows of more than 2^31 - 1 elements");
+  return product(full.shape, 0, full.shape.size() - 1);
+}
+
+void mxfp4_quant_fwd(py::handle x, py::handle codes, py::handle scales) {
+  View xv = validate_tensor("x", x);
+  View cv = validate_codes("codes", codes);
+  View sv = validate_e8m0("scales", scales);
+  require_float("x", xv);
+  check_same_device("codes", cv, xv, "x");
+  check_same_device("scales", sv, xv, "x");
+  const int64_t rows = check_mxfp4_rows(xv, "x", cv);
+  check_mxfp4_pair("x", cv, sv);
+  const Launch launch(xv.device_index);
+  check_launch("launch_mxfp4_quant_fwd",
+               launch_mxfp4_quant_fwd((const void*)xv.ptr, (uint8_t*)cv.ptr, (uint8_t*)sv.ptr, rows, xv.shape.back(),
+                                      xv.dtype, launch.st));
+}
+
+void mxfp4_dequant_fwd(py::handle codes, py::handle scales, py::handle out) {
+  View cv = validate_codes("codes", codes);
+  View sv = validate_e8m0("scales", scales);
+  View ov = validate_tensor("out", out);
+  require_float("out", ov);
+  check_same_device("scales", sv, cv, "codes");
+  check_same_device("out", ov, cv, "codes");
+  check_mxfp4_pair("the", cv, sv);
+  const int64_t rows = check_mxfp4_rows(ov, "out", cv);
+  const Launch launch(cv.device_index);
+  check_launch("launch_mxfp4_dequant_fwd",
+               launch_mxfp4_dequant_fwd((const void*)cv.ptr, (const void*)sv.ptr, (void*)ov.ptr, rows, ov.shape.back(),
+                                        ov.dtype, launch.st));
+}
+
+void mxfp4_linear_fwd(py::handle x_codes, py::handle x_scales, py::handle w_codes, py::handle w_scales,
+                      py::handle offsets, py::handle y) {
+  View xc = validate_codes("x_codes", x_codes);
+  View xs = validate_e8m0("x_scales", x_scales);
+  View wc = validate_codes("w_codes", w_codes);
+  View ws = validate_e8m0("w_scales", w_scales);
+  std::optional<View> ov;
+  if (!offsets.is_none()) ov = validate_int64_tensor("offsets", offsets);
+  View yv = validate_tensor("y", y);
+  require_float("y", yv);
+  check_same_device("x_scales", xs, xc, "x_codes");
+  check_same_device("w_codes", wc, xc, "x_codes");
+  check_same_device("w_scales", ws, xc, "x_codes");
+  if (ov) check_same_device("offsets", *ov, xc, "x_codes");
+  check_same_device("y", yv, xc, "x_codes");
+  check_mxfp4_pair("x", xc, xs);
+  check_mxfp4_pair("w", wc, ws);
+  if (xc.shape.size() != 2) shape_mismatch("x_codes must be 2-D [rows, 16 * blocks], got " + shape_str(xc.shape));
+  const int64_t experts = ov ? check_offsets(*ov) : 1;
+  const size_t dims = ov ? 3 : 2;
+  if (wc.shape.size() != dims || (ov && wc.shape[0] != experts) || wc.shape.back() != xc.shape[1]) {
+    shape_mismatch(std::string("w_codes must be ") + (ov ? "[num_experts, n, 16 * blocks] with offsets [num_experts + 1]"
+                                                         : "[n, 16 * blocks] without offsets") +
+                   " and have x_codes' blocks; got x_codes=" + shape_str(xc.shape) + ", w_codes=" +
+                   shape_str(wc.shape));
+  }
+  const int64_t rows = xc.shape[0], n = wc.shape[dims - 2], blocks = xs.shape[1];
+  if (yv.shape != std::vector<int64_t>{rows, n}) {
+    shape_mismatch("y shape " + shape_str(yv.shape) + " must be [" + std::to_string(rows) + ", " + std::to_string(n) +
+                   "]");
+  }
+  check_product_sizes(rows, n * dtype_bytes(yv.dtype), blocks * 16);
+  const Launch launch(xc.device_index);
+  check_launch("launch_mxfp4_linear_fwd",
+               launch_mxfp4_linear_fwd((const void*)xc.ptr, (const void*)xs.ptr, (const void*)wc.ptr,
+                                       (const void*)ws.ptr, ov ? (const int64_t*)ov->ptr : nullptr, (void*)yv.ptr,
+                                       rows, experts, n, blocks, yv.dtype, launch.st));
+}
+
 }  // namespace
 
 #include "native_calls.hpp"
@@ -713,6 +970,17 @@ PYBIND11_MODULE(_native, m) {
         "Test hook: the hipStream_t (as an int) the most recent call launched on.");
   m.def("swiglu_fp8_fwd", &swiglu_fp8_fwd, py::arg("gate"), py::arg("up"), py::arg("y_fp8"), py::arg("scale"),
         py::arg("fp8_format"), py::arg("static_scale") = py::none());
+  m.def("moe_permutation_offsets_fwd", &moe_permutation_offsets_fwd, py::arg("topk_indices"),
+        py::arg("permute_index"), py::arg("unpermute_index"), py::arg("expert_offsets"), py::arg("num_experts"));
+  m.def("grouped_linear_fwd", &grouped_linear_fwd, py::arg("x"), py::arg("weight"), py::arg("offsets"), py::arg("y"));
+  m.def("grouped_linear_grad_input", &grouped_linear_grad_input, py::arg("grad_y"), py::arg("weight"),
+        py::arg("offsets"), py::arg("grad_x"));
+  m.def("grouped_linear_grad_weight", &grouped_linear_grad_weight, py::arg("grad_y"), py::arg("x"),
+        py::arg("offsets"), py::arg("grad_weight"));
+  m.def("mxfp4_quant_fwd", &mxfp4_quant_fwd, py::arg("x"), py::arg("codes"), py::arg("scales"));
+  m.def("mxfp4_dequant_fwd", &mxfp4_dequant_fwd, py::arg("codes"), py::arg("scales"), py::arg("out"));
+  m.def("mxfp4_linear_fwd", &mxfp4_linear_fwd, py::arg("x_codes"), py::arg("x_scales"), py::arg("w_codes"),
+        py::arg("w_scales"), py::arg("offsets"), py::arg("y"));
   // The Python API in one call each (native_calls.hpp).
   if (PyModule_AddFunctions(m.ptr(), calls::kMethods) != 0) throw py::error_already_set();
 }

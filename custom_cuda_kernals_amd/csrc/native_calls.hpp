@@ -25,6 +25,7 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/util/DimVector.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 
 namespace {
@@ -415,6 +416,166 @@ inline PyObject* moe_router(PyObject*, PyArgs a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// (topk_indices, num_experts), with the experts' offsets
+inline PyObject* compute_permutation_offsets(PyObject*, PyArgs a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2 || !ordinary_state()) Py_RETURN_NONE;
+  const Input ids(a[0]);
+  const int64_t experts = int_arg(a[1], 256);
+  if (!ids || experts < 0 || ids.dim() != 2 || ids.type() != c10::ScalarType::Long) Py_RETURN_NONE;
+  const int64_t flat[1] = {ids.numel()}, bounds[1] = {experts + 1};
+  const Launch launch(ids.device().index());
+  at::Tensor out[3];
+  allocate(ids.device(),
+           {{flat, c10::ScalarType::Long}, {ids.sizes(), c10::ScalarType::Long}, {bounds, c10::ScalarType::Long}}, out);
+  if (!unchanged(ids)) Py_RETURN_NONE;
+  check_launch("launch_moe_permutation_offsets_fwd",
+               launch_moe_permutation_offsets_fwd((const int64_t*)ids.data(), (int64_t*)out[0].data_ptr(),
+                                                  (int64_t*)out[1].data_ptr(), (int64_t*)out[2].data_ptr(),
+                                                  ids.size(0), ids.size(1), experts, launch.st));
+  return result(std::move(out[0]), std::move(out[1]), std::move(out[2]));
+  END_HANDLE_TH_ERRORS
+}
+
+// int64 [num_experts + 1] beside x, or 0 experts for anything else.
+inline int64_t offsets_experts(const Input& offsets, const Input& x) {
+  return offsets.dim() == 1 && offsets.type() == c10::ScalarType::Long && offsets.device() == x.device() &&
+                 offsets.size(0) >= 2 && offsets.size(0) <= kMaxExperts + 1
+             ? offsets.size(0) - 1
+             : 0;
+}
+
+inline bool product_sizes_ok(int64_t rows, int64_t n_bytes, int64_t k_bytes) {
+  return rows <= INT32_MAX && n_bytes <= kMaxRowBytes && k_bytes <= kMaxRowBytes;
+}
+
+// (x, weight, offsets), (grad_y, weight, offsets) or (grad_y, x, offsets): the
+// product, the gradient of x or that of the weight.
+enum class Grouped { kLinear, kGradInput, kGradWeight };
+template <Grouped WHAT>
+inline PyObject* grouped_linear(PyObject*, PyArgs a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (n_args != 3 || !ordinary_state()) Py_RETURN_NONE;
+  const Input x(a[0]), w(a[1]), offsets(a[2]);
+  if (!x || !w || !offsets || float_tag(x) < 0 || w.type() != x.type() || w.device() != x.device() || x.dim() != 2) {
+    Py_RETURN_NONE;
+  }
+  const int64_t experts = offsets_experts(offsets, x), rows = x.size(0);
+  const int32_t dt = float_tag(x);
+  constexpr bool kWeight = WHAT == Grouped::kGradWeight, kLinear = WHAT == Grouped::kLinear;
+  if (experts == 0 || w.dim() != (kWeight ? 2 : 3) || w.size(0) != (kWeight ? rows : experts)) Py_RETURN_NONE;
+  if (!kWeight && x.size(1) != w.size(kLinear ? 2 : 1)) Py_RETURN_NONE;
+  const int64_t n = kWeight ? x.size(1) : w.size(1), k = kWeight ? w.size(1) : w.size(2);
+  if (!product_sizes_ok(rows, n * dtype_bytes(dt), k * dtype_bytes(dt))) Py_RETURN_NONE;
+  const int64_t grad_weight[3] = {experts, n, k}, by_rows[2] = {rows, kLinear ? n : k};
+  const Launch launch(x.device().index());
+  at::Tensor out[1];
+  allocate(x.device(), {{kWeight ? c10::IntArrayRef(grad_weight) : c10::IntArrayRef(by_rows), x.type()}}, out);
+  if (!unchanged(x, w, offsets)) Py_RETURN_NONE;
+  const int64_t* at = (const int64_t*)offsets.data();
+  void* to = out[0].data_ptr();
+  if constexpr (kLinear) {
+    check_launch("launch_grouped_linear_fwd",
+                 launch_grouped_linear_fwd(x.data(), w.data(), at, to, rows, experts, n, k, dt, launch.st));
+  } else if constexpr (kWeight) {
+    check_launch("launch_grouped_linear_grad_weight",
+                 launch_grouped_linear_grad_weight(x.data(), w.data(), at, to, rows, experts, n, k, dt, launch.st));
+  } else {
+    check_launch("launch_grouped_linear_grad_input",
+                 launch_grouped_linear_grad_input(x.data(), w.data(), at, to, rows, experts, n, k, dt, launch.st));
+  }
+  return result(std::move(out[0]));
+  END_HANDLE_TH_ERRORS
+}
+
+// (x)
+inline PyObject* mxfp4_quant(PyObject*, PyArgs a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 1 || !ordinary_state()) Py_RETURN_NONE;
+  const Input x(a[0]);
+  if (!x || float_tag(x) < 0 || x.dim() < 1 || x.size(-1) > INT32_MAX) Py_RETURN_NONE;
+  const int64_t width = x.size(-1), blocks = (width + 31) / 32;
+  c10::DimVector codes(x.sizes()), scales(x.sizes());
+  codes.back() = 16 * blocks;
+  scales.back() = blocks;
+  const Launch launch(x.device().index());
+  at::Tensor out[2];
+  allocate(x.device(), {{codes, c10::ScalarType::Byte}, {scales, c10::ScalarType::Float8_e8m0fnu}}, out);
+  if (!unchanged(x)) Py_RETURN_NONE;
+  check_launch("launch_mxfp4_quant_fwd",
+               launch_mxfp4_quant_fwd(x.data(), (uint8_t*)out[0].data_ptr(), (uint8_t*)out[1].data_ptr(),
+                                      x.numel() / width, width, float_tag(x), launch.st));
+  return result(std::move(out[0]), std::move(out[1]));
+  END_HANDLE_TH_ERRORS
+}
+
+// uint8 codes [..., 16 * blocks] and their scales [..., blocks].
+inline bool mxfp4_pair(const Input& codes, const Input& scales) {
+  return codes.type() == c10::ScalarType::Byte && scales.type() == c10::ScalarType::Float8_e8m0fnu &&
+         codes.device() == scales.device() && codes.dim() >= 1 && codes.dim() == scales.dim() &&
+         codes.size(-1) == 16 * scales.size(-1) &&
+         codes.sizes().slice(0, codes.dim() - 1) == scales.sizes().slice(0, codes.dim() - 1);
+}
+
+// The tag of torch.float32 / float16 / bfloat16, -1 for anything else.
+inline int32_t dtype_arg(PyObject* o) {
+  if (!THPDtype_Check(o)) return -1;
+  const int32_t tag = tag_of(reinterpret_cast<THPDtype*>(o)->scalar_type);
+  return tag == F32 || tag == F16 || tag == BF16 ? tag : -1;
+}
+
+// (codes, scales, width, dtype)
+inline PyObject* mxfp4_dequant(PyObject*, PyArgs a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !ordinary_state()) Py_RETURN_NONE;
+  const Input codes(a[0]), scales(a[1]);
+  const int64_t width = int_arg(a[2], INT32_MAX);
+  const int32_t dt = dtype_arg(a[3]);
+  if (!codes || !scales || width < 0 || dt < 0 || !mxfp4_pair(codes, scales) || (width + 31) / 32 != scales.size(-1)) {
+    Py_RETURN_NONE;
+  }
+  c10::DimVector sizes(codes.sizes());
+  sizes.back() = width;
+  const Launch launch(codes.device().index());
+  at::Tensor out[1];
+  allocate(codes.device(), {{sizes, reinterpret_cast<THPDtype*>(a[3])->scalar_type}}, out);
+  if (!unchanged(codes, scales)) Py_RETURN_NONE;
+  check_launch("launch_mxfp4_dequant_fwd",
+               launch_mxfp4_dequant_fwd(codes.data(), scales.data(), out[0].data_ptr(), scales.numel() / scales.size(-1),
+                                        width, dt, launch.st));
+  return result(std::move(out[0]));
+  END_HANDLE_TH_ERRORS
+}
+
+// (x_codes, x_scales, w_codes, w_scales, offsets, out_dtype)
+inline PyObject* mxfp4_linear(PyObject*, PyArgs a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (n_args != 6 || !ordinary_state()) Py_RETURN_NONE;
+  const Input x(a[0]), xs(a[1]), w(a[2]), ws(a[3]);
+  const bool grouped = a[4] != Py_None;
+  const Input offsets(grouped ? a[4] : a[0]);
+  const int32_t dt = dtype_arg(a[5]);
+  if (!x || !xs || !w || !ws || !offsets || dt < 0 || !mxfp4_pair(x, xs) || !mxfp4_pair(w, ws) ||
+      w.device() != x.device() || x.dim() != 2 || w.dim() != (grouped ? 3 : 2) || w.size(-1) != x.size(1)) {
+    Py_RETURN_NONE;
+  }
+  const int64_t experts = grouped ? offsets_experts(offsets, x) : 1;
+  if (experts == 0 || (grouped && w.size(0) != experts)) Py_RETURN_NONE;
+  const int64_t rows = x.size(0), n = w.size(-2), blocks = xs.size(1);
+  if (!product_sizes_ok(rows, n * dtype_bytes(dt), blocks * 16)) Py_RETURN_NONE;
+  const int64_t sizes[2] = {rows, n};
+  const Launch launch(x.device().index());
+  at::Tensor out[1];
+  allocate(x.device(), {{sizes, reinterpret_cast<THPDtype*>(a[5])->scalar_type}}, out);
+  if (!unchanged(x, xs, w, ws, offsets)) Py_RETURN_NONE;
+  check_launch("launch_mxfp4_linear_fwd",
+               launch_mxfp4_linear_fwd(x.data(), xs.data(), w.data(), ws.data(),
+                                       grouped ? (const int64_t*)offsets.data() : nullptr, out[0].data_ptr(), rows,
+                                       experts, n, blocks, dt, launch.st));
+  return result(std::move(out[0]));
+  END_HANDLE_TH_ERRORS
+}
+
 using FastCall = PyObject* (*)(PyObject*, PyArgs, Py_ssize_t);
 template <FastCall F>
 PyCFunction as_method() {
@@ -432,6 +593,13 @@ inline PyMethodDef kMethods[] = {
     {"token_combine_call", as_method<token_combine>(), METH_FASTCALL, nullptr},
     {"compute_permutation_call", as_method<compute_permutation>(), METH_FASTCALL, nullptr},
     {"moe_router_call", as_method<moe_router>(), METH_FASTCALL, nullptr},
+    {"compute_permutation_offsets_call", as_method<compute_permutation_offsets>(), METH_FASTCALL, nullptr},
+    {"grouped_linear_call", as_method<grouped_linear<Grouped::kLinear>>(), METH_FASTCALL, nullptr},
+    {"grouped_linear_grad_input_call", as_method<grouped_linear<Grouped::kGradInput>>(), METH_FASTCALL, nullptr},
+    {"grouped_linear_grad_weight_call", as_method<grouped_linear<Grouped::kGradWeight>>(), METH_FASTCALL, nullptr},
+    {"mxfp4_quant_call", as_method<mxfp4_quant>(), METH_FASTCALL, nullptr},
+    {"mxfp4_dequant_call", as_method<mxfp4_dequant>(), METH_FASTCALL, nullptr},
+    {"mxfp4_linear_call", as_method<mxfp4_linear>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

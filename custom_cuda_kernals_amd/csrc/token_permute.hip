@@ -907,6 +907,15 @@ __device__ inline void perm_rank_chunk(const int64_t* __restrict__ ids, int64_t 
   }
 }
 
+// The first chunk's bases are where each expert's entries begin: workgroup 0
+// stores them where the caller wants them. Its threads read their own base only
+// (perm_rank_chunk adds to it behind a barrier).
+__device__ inline void perm_store_offsets(const uint32_t* base, int nb, int64_t* __restrict__ expert_offsets) {
+  if (expert_offsets != nullptr && blockIdx.x == 0 && (int)threadIdx.x < nb) {
+    expert_offsets[threadIdx.x] = (int64_t)base[threadIdx.x];
+  }
+}
+
 // One launch: workgroup c owns the entries [c * chunk, (c + 1) * chunk) in
 // tiles of kPermThreads, and counts all n ids per bucket in LDS, those before
 // its chunk (before) and the others (after), one LDS atomic per id. Each
@@ -924,7 +933,8 @@ template <bool kCombine>
 __global__ __launch_bounds__(kPermThreads) void moe_permutation(const int64_t* __restrict__ ids, int64_t n, int64_t k,
                                                                 int n_experts, int64_t chunk,
                                                                 int64_t* __restrict__ permute_index,
-                                                                int64_t* __restrict__ unpermute_index) {
+                                                                int64_t* __restrict__ unpermute_index,
+                                                                int64_t* __restrict__ expert_offsets) {
   // before = sides[0], after = sides[1]
   __shared__ uint32_t sides[2 * kPermBuckets], base[kPermBuckets];
   __shared__ PermTile tile;
@@ -964,6 +974,7 @@ __global__ __launch_bounds__(kPermThreads) void moe_permutation(const int64_t* _
   __syncthreads();
   if (tid < 64) perm_bases(after, before, base, nb, tid);
   __syncthreads();
+  perm_store_offsets(base, nb, expert_offsets);
   perm_rank_chunk<true>(ids, own, k, n_experts, c0, c1, base, tile, permute_index, unpermute_index);
 }
 
@@ -1018,7 +1029,8 @@ __global__ __launch_bounds__(kPermThreads) void moe_permutation_count(const int6
 __global__ __launch_bounds__(kPermThreads) void moe_permutation_rank(const int64_t* __restrict__ ids, int64_t n,
                                                                      int64_t k, int n_experts, int64_t chunk,
                                                                      const uint32_t* __restrict__ counts,
-                                                                     int64_t* __restrict__ unpermute_index) {
+                                                                     int64_t* __restrict__ unpermute_index,
+                                                                     int64_t* __restrict__ expert_offsets) {
   __shared__ uint32_t after[kPermBuckets], before[kPermBuckets], base[kPermBuckets];
   __shared__ PermTile tile;
   const int tid = threadIdx.x;
@@ -1051,7 +1063,13 @@ __global__ __launch_bounds__(kPermThreads) void moe_permutation_rank(const int64
   __syncthreads();
   if (tid < 64) perm_bases(after, before, base, nb, tid);
   __syncthreads();
+  perm_store_offsets(base, nb, expert_offsets);
   perm_rank_chunk<false>(ids, own, k, n_experts, c0, c1, base, tile, nullptr, unpermute_index);
+}
+
+// No entries: every expert's begin at 0.
+__global__ __launch_bounds__(512) void zero_offsets(int64_t* __restrict__ expert_offsets, int n) {
+  if ((int)threadIdx.x < n) expert_offsets[threadIdx.x] = 0;
 }
 
 __global__ __launch_bounds__(256) void moe_permutation_invert(const int64_t* __restrict__ unpermute_index, int64_t n,
@@ -1097,14 +1115,18 @@ extern "C" int32_t launch_token_combine_checked_fwd(const void* expert_output, c
                  n_expert_rows, static_cast<hipStream_t>(stream));
 }
 
-extern "C" int32_t launch_moe_permutation_fwd(const int64_t* topk_indices, int64_t* permute_index,
-                                              int64_t* unpermute_index, int64_t n_tokens, int64_t k,
-                                              int64_t num_experts, void* stream) {
+namespace {
+int32_t permutation(const int64_t* topk_indices, int64_t* permute_index, int64_t* unpermute_index,
+                    int64_t* expert_offsets, int64_t n_tokens, int64_t k, int64_t num_experts, void* stream) {
   if (n_tokens < 0 || k < 0 || num_experts < 1 || num_experts > kPermMaxExperts) return (int32_t)hipErrorInvalidValue;
   if (k > 0 && n_tokens > INT32_MAX / k) return (int32_t)hipErrorInvalidValue;  // positions are 32-bit
   const int64_t n = n_tokens * k;
-  if (n == 0) return (int32_t)hipSuccess;
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (n == 0) {
+    if (expert_offsets == nullptr) return (int32_t)hipSuccess;
+    zero_offsets<<<1, 512, 0, st>>>(expert_offsets, (int)num_experts + 1);
+    return launch_status();
+  }
   if (n >= kPermSplitMin) {
     int64_t chunk = kPermSplitChunk;
     if ((n + chunk - 1) / chunk > kPermSplitMaxGroups) {
@@ -1116,7 +1138,7 @@ extern "C" int32_t launch_moe_permutation_fwd(const int64_t* topk_indices, int64
     uint32_t* counts = reinterpret_cast<uint32_t*>(permute_index);
     moe_permutation_count<<<groups, kPermThreads, 0, st>>>(topk_indices, n, (int)num_experts, chunk, counts);
     moe_permutation_rank<<<groups, kPermThreads, 0, st>>>(topk_indices, n, k, (int)num_experts, chunk, counts,
-                                                          unpermute_index);
+                                                          unpermute_index, expert_offsets);
     const int64_t blocks = (n + 255) / 256;
     moe_permutation_invert<<<(unsigned)(blocks < 2048 ? blocks : 2048), 256, 0, st>>>(unpermute_index, n, k,
                                                                                      permute_index);
@@ -1128,10 +1150,24 @@ extern "C" int32_t launch_moe_permutation_fwd(const int64_t* topk_indices, int64
   const unsigned grid = (unsigned)((n + chunk - 1) / chunk);
   if (k <= 2) {
     moe_permutation<true><<<grid, kPermThreads, 0, st>>>(topk_indices, n, k, (int)num_experts, chunk, permute_index,
-                                                         unpermute_index);
+                                                         unpermute_index, expert_offsets);
   } else {
     moe_permutation<false><<<grid, kPermThreads, 0, st>>>(topk_indices, n, k, (int)num_experts, chunk,
-                                                          permute_index, unpermute_index);
+                                                          permute_index, unpermute_index, expert_offsets);
   }
   return launch_status();
+}
+}  // namespace
+
+extern "C" int32_t launch_moe_permutation_fwd(const int64_t* topk_indices, int64_t* permute_index,
+                                              int64_t* unpermute_index, int64_t n_tokens, int64_t k,
+                                              int64_t num_experts, void* stream) {
+  return permutation(topk_indices, permute_index, unpermute_index, nullptr, n_tokens, k, num_experts, stream);
+}
+
+extern "C" int32_t launch_moe_permutation_offsets_fwd(const int64_t* topk_indices, int64_t* permute_index,
+                                                      int64_t* unpermute_index, int64_t* expert_offsets,
+                                                      int64_t n_tokens, int64_t k, int64_t num_experts,
+                                                      void* stream) {
+  return permutation(topk_indices, permute_index, unpermute_index, expert_offsets, n_tokens, k, num_experts, stream);
 }

@@ -52,8 +52,8 @@ def token_combine(expert_output: torch.Tensor, unpermute_index: torch.Tensor, we
     return combined
 
 
-def compute_permutation(topk_indices: torch.Tensor, num_experts: int | None = None
-                        ) -> tuple[torch.Tensor, torch.Tensor]:
+def compute_permutation(topk_indices: torch.Tensor, num_experts: int | None = None, return_offsets: bool = False
+                        ) -> tuple[torch.Tensor, ...]:
     """From ``topk_indices [T, k]`` (expert per token and slot): ``permute_index
     [T*k]`` (source token of each expert-sorted slot; ties keep token order)
     and ``unpermute_index [T, k]`` (the sorted slot each assignment went to).
@@ -61,7 +61,14 @@ def compute_permutation(topk_indices: torch.Tensor, num_experts: int | None = No
     With ``num_experts`` (at most 256; ids outside ``[0, num_experts)`` are
     ordered after every expert) this is one HIP kernel, a stable counting sort;
     without it, the reference's torch ops (a stable argsort and its inverse,
-    baselines/token_permute.py:55-70) on the tensor's device."""
+    baselines/token_permute.py:55-70) on the tensor's device.
+
+    ``return_offsets`` (with ``num_experts``) returns a third tensor, int64
+    ``[num_experts + 1]``: expert ``e`` has the sorted slots
+    ``offsets[e] .. offsets[e + 1]``, as ``grouped_linear`` takes them. The same
+    launches write it."""
+    if return_offsets:
+        return _permutation_with_offsets(topk_indices, num_experts)
     if num_experts is not None:
         # The ordinary call in one native call; None: the long way below, which raises the errors.
         out = native.compute_permutation_call(topk_indices, num_experts)
@@ -78,3 +85,18 @@ def compute_permutation(topk_indices: torch.Tensor, num_experts: int | None = No
     inverse = torch.empty_like(order)
     inverse[order] = torch.arange(t * k, device=topk_indices.device)
     return permute_index, inverse.reshape(t, k)
+
+
+def _permutation_with_offsets(topk_indices: torch.Tensor, num_experts: int | None) -> tuple[torch.Tensor, ...]:
+    if num_experts is None:
+        raise ValueError("return_offsets needs num_experts")
+    # The ordinary call in one native call; None: the long way below, which raises the errors.
+    out = native.compute_permutation_offsets_call(topk_indices, num_experts)
+    if out is not None:
+        return out
+    t, k = topk_indices.shape
+    permute_index = torch.empty(t * k, dtype=torch.int64, device=topk_indices.device)
+    unpermute_index = torch.empty((t, k), dtype=torch.int64, device=topk_indices.device)
+    offsets = torch.empty(max(int(num_experts), 0) + 1, dtype=torch.int64, device=topk_indices.device)
+    native.moe_permutation_offsets_fwd(topk_indices, permute_index, unpermute_index, offsets, int(num_experts))
+    return permute_index, unpermute_index, offsets

@@ -198,6 +198,68 @@ int32_t launch_moe_router_fwd(const void* logits, float* topk_weights, int64_t* 
 int32_t launch_moe_permutation_fwd(const int64_t* topk_indices, int64_t* permute_index, int64_t* unpermute_index,
                                    int64_t n_tokens, int64_t k, int64_t num_experts, void* stream);
 
+/* As launch_moe_permutation_fwd, and expert_offsets int64 [num_experts + 1] gets
+ * where each expert's entries begin in that order: expert e has the positions
+ * [expert_offsets[e], expert_offsets[e + 1]). Written without entries too (zeros).
+ * No reference counterpart. */
+int32_t launch_moe_permutation_offsets_fwd(const int64_t* topk_indices, int64_t* permute_index,
+                                           int64_t* unpermute_index, int64_t* expert_offsets, int64_t n_tokens,
+                                           int64_t k, int64_t num_experts, void* stream);
+
+/* ---- Expert products (no reference counterpart): the linear layers of a
+ * mixture-of-experts FFN on rows in expert order, and their gradients. One dtype
+ * (F32, F16 or BF16) for all tensors, sums in float32 (fp32: MFMA products and
+ * sums), one rounding at the end. offsets: int64 [num_experts + 1] device memory,
+ * not decreasing, as launch_moe_permutation_offsets_fwd writes it: rows
+ * [offsets[e], offsets[e + 1]) belong to expert e. Rows before offsets[0] and from
+ * offsets[num_experts] on belong to none. Whatever the offsets hold, nothing
+ * outside the `rows` rows is read or written; where they decrease, the results are
+ * unspecified. weight: [num_experts, n, k]. rows <= INT32_MAX, num_experts <= 1024
+ * and n, k of at most 4 MiB a row, else hipErrorInvalidValue. Outputs must not
+ * overlap inputs. ---- */
+
+/* y[s] = x[s] * weight[e]^T for each row s of expert e; zeros for rows of none.
+ * x: [rows, k], y: [rows, n]. */
+int32_t launch_grouped_linear_fwd(const void* x, const void* weight, const int64_t* offsets, void* y, int64_t rows,
+                                  int64_t num_experts, int64_t n, int64_t k, int32_t dtype, void* stream);
+
+/* grad_x[s] = grad_y[s] * weight[e]; zeros for rows of no expert.
+ * grad_y: [rows, n], grad_x: [rows, k]. */
+int32_t launch_grouped_linear_grad_input(const void* grad_y, const void* weight, const int64_t* offsets,
+                                         void* grad_x, int64_t rows, int64_t num_experts, int64_t n, int64_t k,
+                                         int32_t dtype, void* stream);
+
+/* grad_weight[e] = sum over the rows s of expert e of grad_y[s]^T x[s]; zeros for
+ * an expert without rows (rows may be 0). grad_weight: [num_experts, n, k]. */
+int32_t launch_grouped_linear_grad_weight(const void* grad_y, const void* x, const int64_t* offsets,
+                                          void* grad_weight, int64_t rows, int64_t num_experts, int64_t n, int64_t k,
+                                          int32_t dtype, void* stream);
+
+/* ---- MXFP4 (OCP microscaling formats v1.0; no reference counterpart): e2m1 codes,
+ * two a byte with the lower element in the lower half, and one E8M0 scale byte
+ * (2^(byte - 127), 255: NaN) for each 32 neighbours of a row. With blocks =
+ * ceil(width / 32), codes are [rows, 16 * blocks] and scales [rows, blocks]; the
+ * codes of elements past the row's width are zeros. ---- */
+
+/* scale = 2^(floor(log2(max |x|)) - 2) of the block, at least 2^-127; codes of
+ * x / scale to nearest even, saturating at 6. A block that holds a NaN or an
+ * infinity gets the scale byte 255 and zero codes. codes: 4-byte aligned, else
+ * hipErrorInvalidValue. */
+int32_t launch_mxfp4_quant_fwd(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t width,
+                               int32_t dtype, void* stream);
+
+/* out[r][i] = code * scale, [rows, width] of dtype, rounded once. */
+int32_t launch_mxfp4_dequant_fwd(const void* codes, const void* scales, void* out, int64_t rows, int64_t width,
+                                 int32_t dtype, void* stream);
+
+/* y[s] = x[s] * w[e]^T of the values that codes and scales stand for, sums in
+ * float32, y [rows, n] of dtype. x: codes [rows, 16 * blocks], scales [rows, blocks];
+ * w: codes [num_experts, n, 16 * blocks], scales [num_experts, n, blocks]. offsets as
+ * above, or NULL with num_experts == 1 for a dense product. */
+int32_t launch_mxfp4_linear_fwd(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales,
+                                const int64_t* offsets, void* y, int64_t rows, int64_t num_experts, int64_t n,
+                                int64_t blocks, int32_t dtype, void* stream);
+
 /* ---- Diagnostics (no reference counterpart): device-side checks of the
  * arithmetic shortcuts used on the FP8 fast path. ---- */
 
