@@ -15,35 +15,59 @@
 namespace cck {
 namespace {
 
-template <class T, class C, class P, class Q, int WP, int WQ, int FP, int FQ, bool DIRECT>
-__global__ __launch_bounds__(WP* WQ * 64, DIRECT ? 2 : 1) void grouped_weights(const char* __restrict__ grad,
+// An expert's tiles take as long as it has rows, so every XCD gets a share of each
+// expert's where there are enough of them to share (room: up to a multiple of 8, at which
+// the next expert begins); else each takes a run of experts. With a run of all tiles each,
+// one expert an XCD, eight experts of 8192 unevenly routed rows took 1255 us in place of 864.
+constexpr int kTilesApart = 64;
+__host__ __device__ constexpr int weights_room(int each) { return each < kTilesApart ? each : (each + 7) / 8 * 8; }
+
+template <class T, class C, int WP, int WQ, int FP, int FQ, bool DIRECT>
+__global__ __launch_bounds__(WP* WQ * 64, tile_waves(FP* FQ, DIRECT)) void grouped_weights(const char* __restrict__ grad,
                                                               const char* __restrict__ x,
                                                               const int64_t* __restrict__ offsets,
                                                               char* __restrict__ out, int64_t rows, int n, int k,
                                                               int tiles_p, int tiles_q) {
-  using Prod = Product<T, P, Q, NoScales, NoScales, WP, WQ, FP, FQ, DIRECT>;
-  constexpr int BP = WP * FP * 16, BQ = WQ * FQ * 16;
-  __shared__ __attribute__((aligned(1024))) char lds0[Prod::kStage];
-  __shared__ __attribute__((aligned(1024))) char lds1[Prod::kStage];
+  constexpr int BP = WP * FP * 16, BQ = WQ * FQ * 16, NW = WP * WQ, kStep = DIRECT ? 128 : 64;
+  using P = ColOperand<T, BP, NW, kStep>;
+  using Q = ColOperand<T, BQ, NW, kStep>;
+  using Prod = Product<T, P, Q, NoScales, NoScales, WP, WQ, FP, FQ, kStep>;
+  __shared__ __attribute__((aligned(1024))) char lds[Prod::kLds];
 
-  const int each = tiles_p * tiles_q;
-  const int t = xcd_contiguous(blockIdx.x, gridDim.x), e = t / each;
+  const int each = tiles_p * tiles_q, room = weights_room(each);
+  int e, t;
+  if (room >= kTilesApart) {
+    e = blockIdx.x / room;
+    t = xcd_contiguous(blockIdx.x - e * room, room);
+    if (t >= each) return;
+  } else {
+    t = xcd_contiguous(blockIdx.x, gridDim.x);
+    e = t / each;
+    t -= e * each;
+  }
   int tp, tq;
-  tile_order(t - e * each, tiles_p, tiles_q, &tp, &tq);
-  const int64_t lo = clamp_row(offsets[e], rows), hi = clamp_row(offsets[e + 1], rows);
+  tile_order(t, tiles_p, tiles_q, &tp, &tq);
+  const int64_t lo = uniform(clamp_row(offsets[e], rows)), hi = uniform(clamp_row(offsets[e + 1], rows));
   const int64_t length = hi > lo ? hi - lo : 0;
   const int p0 = tp * BP, q0 = tq * BQ;
   const int height = n - p0 < BP ? n - p0 : BP, width = k - q0 < BQ ? k - q0 : BQ;
   P p(grad + (lo * n + p0) * T::kBytes, (int64_t)n * T::kBytes, height, length);
   Q q(x + (lo * k + q0) * T::kBytes, (int64_t)k * T::kBytes, width, length);
+  const int steps = (int)((length + P::kDepth - 1) / P::kDepth), wave = wave_of<NW>();
+  const int wp0 = (wave / WQ) * FP * 16, wq0 = (wave % WQ) * FQ * 16;
+  char* const to = out + (((int64_t)e * n + p0) * k + q0) * C::kBytes;
+  if (steps == 0) {
+    store_zeros<C, NW>(to, k, height, width);
+    return;
+  }
+  if (wp0 >= height || wq0 >= width) {
+    Prod::idle(p, q, NoScales(), NoScales(), steps, (LdsPtr)lds);
+    return;
+  }
   f32x4 acc[FP][FQ] = {};
-  constexpr int kDepth = kRowBytes / T::kBytes;
-  Prod::run(p, q, NoScales(), NoScales(), (int)((length + kDepth - 1) / kDepth), (LdsPtr)lds0, (LdsPtr)lds1, acc);
-
-  const int wave = threadIdx.x >> 6;
-  const bool aligned = k % C::VEC == 0 && aligned16(out);
-  store_tile<C, false>(acc, out + (((int64_t)e * n + p0) * k + q0) * T::kBytes, k,
-                                       (wave / WQ) * FP * 16, (wave % WQ) * FQ * 16, height, width, aligned);
+  Prod::run(p, q, NoScales(), NoScales(), steps, (LdsPtr)lds, wp0, wq0, acc);
+  store_tile<C, false, FP, FQ, Prod::kLds / NW>(acc, (LdsPtr)lds + wave * (Prod::kLds / NW), to, k, wp0, wq0, height,
+                                                width);
 }
 
 // fn(element type, its storage codec) for a dtype tag.
@@ -73,8 +97,22 @@ int32_t grouped_rows(const void* x, const void* w, const int64_t* offsets, void*
     const RowsArgs a = {static_cast<const char*>(x), static_cast<const char*>(w), nullptr, nullptr, offsets,
                         static_cast<char*>(out), rows, length, (int)groups, (int)cols, 0, 0};
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (whole_vectors(x, w, cols, length, T::kBytes)) return launch_rows<T, C, QROWS, 2, 2, 4, 4, true>(a, st);
-    return launch_rows<T, C, QROWS, 2, 2, 4, 4, false>(a, st);
+    if (length * T::kBytes < 16 || (!QROWS && cols * T::kBytes < 16)) {
+      const NarrowArgs n = {a.x, a.w, offsets, a.out, rows, length, 1, QROWS ? length : 1, QROWS ? 1 : cols,
+                            length * cols, 0, cols, length, (int)groups};
+      narrow_rows<C><<<narrow_grid(rows * cols), 256, 0, st>>>(n);
+      return launch_status();
+    }
+    const bool whole = whole_vectors(x, w, cols, length, T::kBytes);
+    if constexpr (QROWS) {
+      return whole ? launch_rows_by_size<T, C, true>(a, st) : launch_rows_by_size<T, C, false>(a, st);
+    } else {
+      if constexpr (T::kAccumulates) {
+        if (whole && wide_tiles(a, 64)) return launch_rows<T, C, false, 2, 2, 8, 8, true>(a, st);
+      }
+      return whole ? launch_rows<T, C, false, 2, 2, 4, 4, true>(a, st)
+                   : launch_rows<T, C, false, 2, 2, 4, 4, false>(a, st);
+    }
   });
 }
 
@@ -83,9 +121,10 @@ int32_t run_weights(const void* grad, const void* x, const int64_t* offsets, voi
                     int64_t n, int64_t k, hipStream_t st) {
   constexpr int BP = WP * FP * 16, BQ = WQ * FQ * 16, NW = WP * WQ;
   const int64_t tiles_p = (n + BP - 1) / BP, tiles_q = (k + BQ - 1) / BQ;
-  if (groups * tiles_p * tiles_q * NW * 64 >= kMaxThreads) return (int32_t)hipErrorInvalidValue;
-  grouped_weights<T, C, ColOperand<T, BP, NW>, ColOperand<T, BQ, NW>, WP, WQ, FP, FQ, DIRECT>
-      <<<(unsigned)(groups * tiles_p * tiles_q), NW * 64, 0, st>>>(
+  if (groups * (tiles_p * tiles_q + 7) * NW * 64 >= kMaxThreads) return (int32_t)hipErrorInvalidValue;
+  const int64_t grid = groups * weights_room((int)(tiles_p * tiles_q));
+  grouped_weights<T, C, WP, WQ, FP, FQ, DIRECT>
+      <<<(unsigned)grid, NW * 64, 0, st>>>(
           static_cast<const char*>(grad), static_cast<const char*>(x), offsets, static_cast<char*>(out), rows, (int)n,
           (int)k, (int)tiles_p, (int)tiles_q);
   return launch_status();
@@ -117,7 +156,18 @@ extern "C" int32_t launch_grouped_linear_grad_weight(const void* grad_y, const v
     using C = decltype(codec);
     if (num_experts <= 0 || n <= 0 || k <= 0) return (int32_t)hipSuccess;
     if (!sizes_ok(rows, num_experts, n * T::kBytes, k * T::kBytes)) return (int32_t)hipErrorInvalidValue;
+    if (n * T::kBytes < 16 || k * T::kBytes < 16) {
+      const NarrowArgs a = {static_cast<const char*>(grad_y), static_cast<const char*>(x), offsets,
+                            static_cast<char*>(grad_weight), rows, 1, n, 1, k, 0, n, k, 0, (int)num_experts};
+      narrow_weights<C><<<narrow_grid(num_experts * n * k), 256, 0, st>>>(a);
+      return launch_status();
+    }
     if (whole_vectors(grad_y, x, n, k, T::kBytes)) {
+      if constexpr (T::kAccumulates) {
+        if (rows >= 256 * num_experts && num_experts * ((n + 255) / 256) * ((k + 255) / 256) >= 256) {
+          return run_weights<T, C, 2, 2, 8, 8, true>(grad_y, x, offsets, grad_weight, rows, num_experts, n, k, st);
+        }
+      }
       return run_weights<T, C, 2, 2, 4, 4, true>(grad_y, x, offsets, grad_weight, rows, num_experts, n, k, st);
     }
     return run_weights<T, C, 2, 2, 4, 4, false>(grad_y, x, offsets, grad_weight, rows, num_experts, n, k, st);

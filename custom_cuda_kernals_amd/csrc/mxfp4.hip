@@ -18,6 +18,22 @@ constexpr int kBlock = 32;    // elements of a scale
 constexpr int kQuarter = 8;   // elements of a thread: four threads share a block
 constexpr int kThreads = 256;
 
+// The first `bytes` (below 16) at p, zeros after them. BYTES: of an element.
+template <int BYTES>
+__device__ inline u32x4 load_short(const char* p, int bytes) {
+  u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 16 / BYTES; ++i) {
+    if (i * BYTES < bytes) {
+      uint32_t e;
+      if constexpr (BYTES == 4) e = *reinterpret_cast<const u32_any*>(p + i * 4);
+      if constexpr (BYTES == 2) e = *reinterpret_cast<const u16_any*>(p + i * 2);
+      v[i * BYTES / 4] |= e << (8 * (i * BYTES % 4));
+    }
+  }
+  return v;
+}
+
 // Eight elements from element `first` of x, of which `count` (0 .. 8) exist; zeros after them.
 template <class C, bool WHOLE>
 __device__ inline void load_quarter(const void* x, int64_t first, int count, float (&f)[kQuarter]) {
@@ -29,7 +45,7 @@ __device__ inline void load_quarter(const void* x, int64_t first, int count, flo
       w = ld_stream(reinterpret_cast<const u32x4*>(p) + v);
     } else {
       const int part = (count - v * C::VEC) * C::kBytes;
-      w = load_part<C::kBytes>(p + v * 16, part < 0 ? 0 : part);
+      w = part >= 16 ? *reinterpret_cast<const u32x4_any*>(p + v * 16) : load_short<C::kBytes>(p + v * 16, part);
     }
     float g[C::VEC];
     C::unpack(w, g);
@@ -195,7 +211,6 @@ extern "C" int32_t launch_mxfp4_linear_fwd(const void* x_codes, const void* x_sc
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool whole = blocks % 4 == 0 && host_aligned(x_codes, 16) && host_aligned(w_codes, 16) &&
                        host_aligned(x_scales, 4) && host_aligned(w_scales, 4);
-    if (whole) return launch_rows<ElemFP4, C, true, 2, 2, 4, 4, true>(a, st);
-    return launch_rows<ElemFP4, C, true, 2, 2, 4, 4, false>(a, st);
+    return whole ? launch_rows_by_size<ElemFP4, C, true>(a, st) : launch_rows_by_size<ElemFP4, C, false>(a, st);
   });
 }

@@ -235,3 +235,61 @@ def test_gradients_against_differences():
         a[e, r, c] += 1
         b[e, r, c] -= 1
         assert (loss(x, a) - loss(x, b)) / 2 == float(grad_w[e, r, c])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=IDS[1:])
+@pytest.mark.parametrize("k", [8, 64, 72, 136, 200, 264])
+def test_large_tiles_forward(k, dtype):
+    """Rows and columns enough for the largest tiles: full, cut in rows and in columns at every part of one; from one
+    step of the contracted index to five, odd and even."""
+    sizes, n = [700, 129, 0, 1, 1100, 641, 40], 7440
+    offsets = _offsets(sizes, 3)
+    rows = int(offsets[-1]) + 30
+    x, w = _ints((rows, k), 4, dtype, k), _ints((len(sizes), n, k), 4, dtype, k + 1)
+    got = K.grouped_linear(x.cuda(), w.cuda(), offsets.cuda()).cpu()
+    want = _rounded(products.grouped_linear(_np(x), _np(w), offsets.numpy()), dtype)
+    assert torch.equal(got, want), (got != want).nonzero()[:4].tolist()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=IDS[1:])
+@pytest.mark.parametrize("n", [8, 64, 72, 136, 200, 264])
+def test_large_tiles_grad_input(n, dtype):
+    sizes, k = [700, 129, 0, 1, 1100, 641, 40], 7440
+    offsets = _offsets(sizes, 3)
+    rows = int(offsets[-1]) + 30
+    g, w = _ints((rows, n), 4, dtype, n), _ints((len(sizes), n, k), 4, dtype, n + 1)
+    got = K.grouped_linear_grad_input(g.cuda(), w.cuda(), offsets.cuda()).cpu()
+    want = _rounded(products.grouped_linear_grad_input(_np(g), _np(w), offsets.numpy()), dtype)
+    assert torch.equal(got, want), (got != want).nonzero()[:4].tolist()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=IDS[1:])
+@pytest.mark.parametrize("n,k", [(2064, 2104), (8, 65544), (65544, 8)])
+def test_large_tiles_grad_weight(n, k, dtype):
+    """Experts of 0 to 1000 rows; weights in full and cut tiles, and of few rows or columns."""
+    sizes = [1000, 1, 0, 129, 256] if n * k < 1 << 20 else [520, 0, 330]
+    offsets = _offsets(sizes, 2)
+    rows = max(int(offsets[-1]) + 5, 256 * len(sizes))
+    g, x = _ints((rows, n), 4, dtype, n), _ints((rows, k), 4, dtype, k)
+    got = K.grouped_linear_grad_weight(g.cuda(), x.cuda(), offsets.cuda()).cpu()
+    want = _rounded(products.grouped_linear_grad_weight(_np(g), _np(x), offsets.numpy()), dtype)
+    assert torch.equal(got, want), (got != want).nonzero()[:4].tolist()
+
+
+@pytest.mark.parametrize("per", [1, 8, 16, 17, 32, 33, 64, 127, 129])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_rows_a_group(per, dtype):
+    """Either side of the average group sizes that other kernels take, with uneven groups."""
+    sizes = [0, 2 * per, per, per + 1, per - 1]
+    _check_ints(sizes, 200, 264, dtype, seed=per)
+    _check_ints(sizes, 67, 75, dtype, seed=per)
+
+
+def test_large_tiles_twice_alike():
+    """No order of the sums depends on the launch: two calls agree bit for bit."""
+    x, w = _normal((2600, 1000), torch.bfloat16, 1).cuda(), _normal((1, 5208, 1000), torch.bfloat16, 2).cuda()
+    o = torch.tensor([0, 2600], device="cuda")
+    y = K.grouped_linear(x, w, o)
+    assert torch.equal(y, K.grouped_linear(x, w, o))
+    gw = K.grouped_linear_grad_weight(y, x, o)
+    assert torch.equal(gw, K.grouped_linear_grad_weight(y, x, o))

@@ -211,3 +211,21 @@ def test_nothing_to_sum():
     c, s = K.mxfp4_quant(torch.zeros(0, 64, device="cuda"))
     wc, ws = K.mxfp4_quant(torch.zeros(5, 64, device="cuda"))
     assert K.mxfp4_linear(c, s, wc, ws).shape == (0, 5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("k", [128, 256, 384, 640])
+def test_large_tiles(k, dtype):
+    """Rows and columns enough for the largest tiles, full and cut; odd and even numbers of steps."""
+    _check_linear([300, 1, 0, 900, 129], 7442, k, dtype, seed=k, first=3, rows=1500, low=126, high=128)
+
+
+def test_large_tiles_dense():
+    _check_linear([1930], 6656, 512, torch.bfloat16, seed=2, dense=True, low=126, high=128)
+
+
+@pytest.mark.parametrize("per", [1, 16, 17, 32, 33, 127, 129])
+def test_rows_a_group(per):
+    """Either side of the average group sizes that other kernels take, with uneven groups."""
+    for k in (256, 224):
+        _check_linear([0, 2 * per, per, per + 1, per - 1], 150, k, torch.bfloat16, seed=per, low=126, high=128)
