@@ -436,10 +436,13 @@ struct ColOperand {
   static constexpr int kLds = R * STEP;
   static constexpr int kLoads = R * (STEP / 16) / (NW * 64);
   static_assert(kLoads * NW * 64 == R * (STEP / 16));
-  // 32 bytes apart from row to row, and 128 from lane group to lane group.
+  // 32 bytes apart from row to row, and 128 from lane group to lane group (rows of 128
+  // bytes: from row to row but one, and 64).
   __device__ static int swizzle(int c) {
+    if constexpr (kWide == 8) return ((c >> 1) & 1) << 1 | ((c >> 3) & 1) << 2;
     return T::kBytes == 2 ? (c & 3) << 1 | ((c >> 3) & 1) << 3 : ((c >> 2) & 3) * 4;
   }
+  static_assert(kWide >= 16 || (kWide == 8 && T::kBytes == 2));
   __device__ static int frag_row(int f, int i) { return 16 * f + i; }
 
   const char* base;  // the tile's first column at the current step
@@ -709,7 +712,9 @@ struct Product {
   static constexpr bool kSumsApart = kWide || (kDirect && T::kScaled);
   static constexpr int kParts = kWide ? FP * FQ : FP;
   // In half 1 the reads take the first parts, and the loads all behind the barrier, of both halves.
-  static constexpr int kReadParts = kWide ? 20 : kParts / 4, kMeetPart = kReadParts + (kParts + 15) / 16;
+  static constexpr int kReadParts = kWide ? 20 : (kParts + 3) / 4;
+  static constexpr int kMeetPart = kParts == 2 ? 1 : kReadParts + (kParts + 15) / 16;
+  static_assert(kReadParts <= kMeetPart && kMeetPart < kParts);
   static constexpr int kAskParts = 2 * kParts - kMeetPart;
   // fn(i) for the items i of `items` that part `part` of `parts` takes, spread evenly.
   template <class Fn>
@@ -1049,7 +1054,8 @@ template <class T, class C, bool QROWS, int WP, int WQ, int FP, int FQ, bool DIR
 __global__ __launch_bounds__(WP* WQ * 64, tile_waves(FP* FQ, DIRECT)) void rows_product(RowsArgs a) {
   constexpr int BP = WP * FP * 16, BQ = WQ * FQ * 16, NW = WP * WQ, kStep = DIRECT ? 128 : 64;
   using P = RowOperand<T, BP, NW, false, kStep>;
-  using Q = std::conditional_t<QROWS, RowOperand<T, BQ, NW, true, kStep>, ColOperand<T, BQ, NW, kStep>>;
+  constexpr bool kPerm = QROWS && FQ % 4 == 0;
+  using Q = std::conditional_t<QROWS, RowOperand<T, BQ, NW, kPerm, kStep>, ColOperand<T, BQ, NW, kStep>>;
   using PS = std::conditional_t<T::kScaled, Scales<P, BP, NW, FP, kStep>, NoScales>;
   using QS = std::conditional_t<T::kScaled, Scales<Q, BQ, NW, FQ, kStep>, NoScales>;
   using Prod = Product<T, P, Q, PS, QS, WP, WQ, FP, FQ, kStep>;
@@ -1094,7 +1100,7 @@ __global__ __launch_bounds__(WP* WQ * 64, tile_waves(FP* FQ, DIRECT)) void rows_
   }
   f32x4 acc[FP][FQ] = {};
   Prod::run(p, q, ps, qs, steps, (LdsPtr)lds, p0, q0, acc);
-  store_tile<C, QROWS, FP, FQ, Prod::kLds / NW>(acc, (LdsPtr)lds + wave * (Prod::kLds / NW), out, a.cols, p0, q0,
+  store_tile<C, kPerm, FP, FQ, Prod::kLds / NW>(acc, (LdsPtr)lds + wave * (Prod::kLds / NW), out, a.cols, p0, q0,
                                                 at.count, width);
 }
 
@@ -1440,6 +1446,21 @@ inline bool wide_tiles(const RowsArgs& a, int64_t filled) {
   return a.rows >= filled * a.groups && (a.rows / 256 + a.groups / 2) * ((a.cols + 255) / 256) >= 200;
 }
 
+// Tiles of 128 x 128, or of 64 x 64 where there would be fewer than 192 of those for the
+// 256 CUs (bf16, us, 128 against 64: 8 groups of 64 rows, 2048 x 2048, 144 tiles 31.5
+// against 28.4; 16 of 128, 2048 x 1024, 200 tiles 32.9 against 34.7), and always for fp32,
+// whose products take the matrix cores 16 times as long (13 groups of 77 rows, 1003 x 777:
+// 70.6 against 40.7; 4096 rows, 4096 x 4096: 955 against 980).
+template <class T, class C, bool QROWS, bool WHOLE>
+int32_t launch_rows_small(const RowsArgs& a, hipStream_t st) {
+  if constexpr (T::kBytes != 4) {
+    if ((a.rows / 128 + a.groups / 2 + 1) * ((a.cols + 127) / 128) >= 192) {
+      return launch_rows<T, C, QROWS, 2, 2, 4, 4, WHOLE>(a, st);
+    }
+  }
+  return launch_rows<T, C, QROWS, 2, 2, 2, 2, WHOLE>(a, st);
+}
+
 // Which kernel, for weights that are rows of the contracted index.
 template <class T, class C, bool WHOLE>
 int32_t launch_rows_by_size(const RowsArgs& a, hipStream_t st) {
@@ -1454,7 +1475,7 @@ int32_t launch_rows_by_size(const RowsArgs& a, hipStream_t st) {
   if constexpr (WHOLE && T::kAccumulates) {
     if (wide_tiles(a, 128)) return launch_rows<T, C, true, 2, 2, 8, 8, true>(a, st);
   }
-  return launch_rows<T, C, true, 2, 2, 4, 4, WHOLE>(a, st);
+  return launch_rows_small<T, C, true, WHOLE>(a, st);
 }
 
 // Sizes every kernel here accepts: 32-bit row counts and columns, rows that 32-bit

@@ -293,3 +293,12 @@ def test_large_tiles_twice_alike():
     assert torch.equal(y, K.grouped_linear(x, w, o))
     gw = K.grouped_linear_grad_weight(y, x, o)
     assert torch.equal(gw, K.grouped_linear_grad_weight(y, x, o))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("sizes,n,k", [([2000], 1032, 1064), ([700, 900], 900, 1000), ([40] * 8, 2056, 136),
+                                       ([130, 0, 300], 1001, 517), ([33] * 64, 40, 48)],
+                         ids=lambda v: "x".join(map(str, v))[:20] if isinstance(v, list) else str(v))
+def test_few_tiles_and_many(sizes, n, k, dtype):
+    """Either side of where smaller tiles are taken."""
+    _check_ints(sizes, n, k, dtype, seed=n)
