@@ -58,6 +58,12 @@ def _require_gpu() -> None:
         raise typer.Exit(code=1)
 
 
+def _require_bench(spec) -> None:
+    if not spec.bench_ops:
+        err.print(f"[bold red]bench.py does not time {spec.id}; `compare {spec.id}` does.[/bold red]")
+        raise typer.Exit(code=1)
+
+
 def _help_table() -> None:
     console.print(Panel(f"[bold cyan]custom_cuda_kernals_amd[/bold cyan] v{__version__} — hand-written HIP "
                         "kernels for MI355X behind the reference's C ABI", box=box.ROUNDED, border_style="cyan"))
@@ -137,7 +143,7 @@ def info(op: str = typer.Argument(..., help="Op id (see `list`).")) -> None:
     body.append(f"  C ABI:        {', '.join(s.c_entry_points)} (include/custom_kernels_amd.h)\n")
     body.append(f"  sources:      {', '.join(s.sources)}\n")
     body.append(f"  tests:        {', '.join(s.test_files)}\n")
-    body.append(f"  bench.py ops: {', '.join(s.bench_ops)}\n")
+    body.append(f"  bench.py ops: {', '.join(s.bench_ops) or '-'}\n")
     body.append(f"  reference:    {', '.join(s.reference)}\n")
     console.print(Panel(body, title=f"[bold cyan]{s.number:02d}[/bold cyan] — {s.title}", border_style="cyan"))
 
@@ -207,6 +213,7 @@ def benchmark(op: str = typer.Argument(..., help="Op id (see `list`)."),
     spec = _resolve(op)
     line = None if rerun else load_bench(spec.id)
     if line is None:
+        _require_bench(spec)
         _require_gpu()
         with console.status(f"[cyan]bench.py --ops {','.join(spec.bench_ops)}...[/cyan]"):
             try:
@@ -246,6 +253,7 @@ def visualize(op: str = typer.Argument(..., help="Op id (see `list`)."),
     spec = _resolve(op)
     line = None if rerun else load_bench(spec.id)
     if line is None:
+        _require_bench(spec)
         _require_gpu()
         with console.status("[cyan]no stored result: running bench.py...[/cyan]"):
             line = run_bench(spec.id, spec.bench_ops, 100, 900)

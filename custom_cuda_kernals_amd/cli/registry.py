@@ -203,6 +203,41 @@ def _t_moe_router(device: str) -> Target:
                   2048 * 160 * 4 + 2048 * 6 * 12)
 
 
+def _t_grouped_linear(device: str) -> Target:
+    import torch
+
+    from custom_cuda_kernals_amd.kernels import grouped_linear
+
+    g = _gen(device)
+    experts, per, n, k = 8, 512, 2048, 4096
+    x, w = _rn((experts * per, k), torch.bfloat16, device, g), _rn((experts, n, k), torch.bfloat16, device, g)
+    offsets = torch.arange(0, experts + 1, device=device) * per
+
+    def eager():
+        return torch.cat([a @ b.t() for a, b in zip(x.split(per), w)])
+
+    return Target(lambda: grouped_linear(x, w, offsets), eager, "grouped_linear bf16 8 x 512 rows, 4096 -> 2048",
+                  2 * (x.numel() + w.numel() + experts * per * n))
+
+
+def _t_mxfp4(device: str) -> Target:
+    import torch
+
+    from custom_cuda_kernals_amd.kernels import mxfp4_dequant, mxfp4_linear, mxfp4_quant
+
+    g = _gen(device)
+    rows, n, k = 16, 14336, 4096
+    x = mxfp4_quant(_rn((rows, k), torch.bfloat16, device, g))
+    w = mxfp4_quant(_rn((n, k), torch.bfloat16, device, g))
+    values = mxfp4_dequant(*w, k, torch.bfloat16)
+
+    def eager():
+        return mxfp4_dequant(*x, k, torch.bfloat16) @ values.t()
+
+    return Target(lambda: mxfp4_linear(*x, *w), eager, "mxfp4_linear [16, 4096] x [14336, 4096]",
+                  (rows + n) * k // 32 * 17 + rows * n * 2)
+
+
 _CSRC = "custom_cuda_kernals_amd/csrc/"
 
 REGISTRY: dict[str, OpSpec] = {
@@ -323,7 +358,7 @@ REGISTRY: dict[str, OpSpec] = {
             python_api=("token_gather", "token_combine", "compute_permutation"),
             c_entry_points=("launch_token_gather_fwd", "launch_token_combine_fwd",
                             "launch_token_gather_checked_fwd", "launch_token_combine_checked_fwd",
-                            "launch_moe_permutation_fwd"),
+                            "launch_moe_permutation_fwd", "launch_moe_permutation_offsets_fwd"),
             sources=(_CSRC + "token_permute.hip",), test_files=("tests/test_token_permute_gpu.py",
                                                                  "tests/test_oracle_moe.py"),
             bench_ops=("token_gather", "token_combine_k2", "token_combine_k6", "moe_permutation"),
@@ -344,6 +379,41 @@ REGISTRY: dict[str, OpSpec] = {
             python_api=("moe_router",), c_entry_points=("launch_moe_router_fwd",), sources=(_CSRC + "moe_router.hip",),
             test_files=("tests/test_moe_router_gpu.py", "tests/test_oracle_moe.py"), bench_ops=("moe_router", "moe_router_e8"),
             build_target=_t_moe_router),
+        OpSpec(
+            id="grouped_linear", number=9, title="Products grouped by expert, and their gradients",
+            purpose="The linear layers of a mixture-of-experts FFN on rows in expert order, groups of any size.",
+            formula="y[s] = x[s] w[e]^T; grad_x[s] = grad_y[s] w[e]; grad_w[e] = sum_s grad_y[s]^T x[s]; "
+                    "offsets[e] <= s < offsets[e + 1]",
+            dtypes=("float32", "float16", "bfloat16"),
+            memory_profile="few rows an expert: HBM-bound (the weights, once); many: bound by the matrix cores.",
+            design=("group sizes stay on the GPU: the grid has room for the most tiles the rows can make",
+                    "tiles of 256 x 256, 128 x 128 or 64 x 64, loaded straight into LDS between the products",
+                    "few rows: the contracted index split over a workgroup's waves, each with its own ring in LDS",
+                    "odd widths and alignments through registers, clamped at the load"),
+            target="sums in float32, one rounding; the same bits from every launch",
+            reference=("an addition",),
+            python_api=("grouped_linear", "grouped_linear_grad_input", "grouped_linear_grad_weight"),
+            c_entry_points=("launch_grouped_linear_fwd", "launch_grouped_linear_grad_input",
+                            "launch_grouped_linear_grad_weight"),
+            sources=(_CSRC + "grouped_linear.hip", _CSRC + "tile_product.hpp"),
+            test_files=("tests/test_grouped_linear_gpu.py", "tests/test_expert_layer_gpu.py",
+                        "tests/test_expert_products_use_gpu.py", "tests/test_products_cpu.py"),
+            bench_ops=(), build_target=_t_grouped_linear),
+        OpSpec(
+            id="mxfp4", number=10, title="MXFP4: quantiser, inverse and products",
+            purpose="OCP microscaling FP4: 32 neighbours share a power of two; products dense and grouped by expert.",
+            formula="X = 2^(floor(log2(max |x|)) - 2); code = e2m1(x / X); y[s] = values(x)[s] values(w[e])^T",
+            dtypes=("float32", "float16", "bfloat16"),
+            memory_profile="quantiser and inverse: HBM-bound; products as grouped_linear's, 17 bytes for 32 elements.",
+            design=("a thread a quarter of a block, the maximum by DPP, the hardware's conversion with scale 1",
+                    "products on the scaled matrix instructions, whose operands are the codes and scales as they are"),
+            target="codes, scales and values bit for bit; sums in float32, one rounding",
+            reference=("an addition",), python_api=("mxfp4_quant", "mxfp4_dequant", "mxfp4_linear"),
+            c_entry_points=("launch_mxfp4_quant_fwd", "launch_mxfp4_dequant_fwd", "launch_mxfp4_linear_fwd"),
+            sources=(_CSRC + "mxfp4.hip", _CSRC + "tile_product.hpp"),
+            test_files=("tests/test_mxfp4_gpu.py", "tests/test_expert_layer_gpu.py",
+                        "tests/test_expert_products_use_gpu.py", "tests/test_products_cpu.py"),
+            bench_ops=(), build_target=_t_mxfp4),
     ]
 }
 

@@ -205,3 +205,15 @@ def test_oracle_products_against_a_loop():
     assert np.allclose(products.grouped_linear(x, w, offsets), y, rtol=1e-14, atol=1e-14)
     assert np.allclose(products.grouped_linear_grad_input(g, w, offsets), gx, rtol=1e-14, atol=1e-14)
     assert np.allclose(products.grouped_linear_grad_weight(g, x, offsets), gw, rtol=1e-14, atol=1e-14)
+
+
+def test_cli_names_the_products():
+    from typer.testing import CliRunner
+
+    from custom_cuda_kernals_amd.cli import app as cli_app
+
+    run = CliRunner().invoke
+    for op, entry in (("grouped_linear", "launch_grouped_linear_grad_weight"), ("mxfp4", "launch_mxfp4_linear_fwd")):
+        shown = run(cli_app.app, ["info", op])
+        assert shown.exit_code == 0 and entry in shown.output
+        assert run(cli_app.app, ["benchmark", op, "--rerun"]).exit_code == 1  # bench.py does not time them
