@@ -108,7 +108,7 @@ int32_t grouped_rows(const void* x, const void* w, const int64_t* offsets, void*
       return whole ? launch_rows_by_size<T, C, true>(a, st) : launch_rows_by_size<T, C, false>(a, st);
     } else {
       if constexpr (T::kAccumulates) {
-        if (whole && wide_tiles(a, 64)) return launch_rows<T, C, false, 2, 2, 8, 8, true>(a, st);
+        if (whole && wide_tiles<T>(a)) return launch_rows<T, C, false, 2, 2, 8, 8, true>(a, st);
       }
       return whole ? launch_rows_small<T, C, false, true>(a, st) : launch_rows_small<T, C, false, false>(a, st);
     }
@@ -129,17 +129,18 @@ int32_t run_weights(const void* grad, const void* x, const int64_t* offsets, voi
   return launch_status();
 }
 
-// Tiles of 256 x 256 where experts have 256 rows or more on average and each CU gets a tile
-// (bf16, us, against 128 x 128: 8 experts of 512 rows, 14336 x 4096 592 and 627, of 128 rows
-// 377 and 316); of 64 x 64 where fewer than 96 of 128 x 128 would share the 256 CUs (8192
-// rows, 1024 x 1024, 64 tiles: 54.5 and 67.0; 4 experts of 500 rows, 1024 x 1536, 384 tiles: 15.8
-// and 13.7), and always for fp32 (8192 rows, 1024 x 1024: 174 and 513; 4096 x 4096: 982 and 963).
+// Tiles of 256 x 256 where experts have 768 rows or more on average and each CU gets a tile
+// (bf16, us, against 128 x 128: 8 experts of 1024 rows, 2048 x 1408 65.7 and 67.8, of 512 rows,
+// 2048 x 2048 49.3 and 46.5; one of 4096 rows, 4096 x 4096 98.9 and 131); of 64 x 64 where
+// fewer than 96 of 128 x 128 would share the 256 CUs (8192 rows, 1024 x 1024, 64 tiles: 54.5
+// and 67.0; 4 experts of 500 rows, 1024 x 1536, 384 tiles: 15.8 and 13.7), and always for
+// fp32 (8192 rows, 1024 x 1024: 174 and 513; 4096 x 4096: 982 and 963).
 template <class T, class C, bool WHOLE>
 int32_t run_weights_by_size(const void* grad, const void* x, const int64_t* offsets, void* out, int64_t rows,
                             int64_t groups, int64_t n, int64_t k, hipStream_t st) {
   if constexpr (T::kBytes != 4) {
     if constexpr (WHOLE) {
-      if (rows >= 256 * groups && groups * ((n + 255) / 256) * ((k + 255) / 256) >= 256) {
+      if (rows >= 768 * groups && groups * ((n + 255) / 256) * ((k + 255) / 256) >= 256) {
         return run_weights<T, C, 2, 2, 8, 8, true>(grad, x, offsets, out, rows, groups, n, k, st);
       }
     }

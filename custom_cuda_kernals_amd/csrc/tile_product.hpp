@@ -148,81 +148,75 @@ struct RowTileAt {
   int count, group;
 };
 
-// The number of row tiles of BP rows, and which rows the tile `index` of them
-// holds. Threads hold the groups' tile counts, whose prefix sums say where each
-// group's tiles begin. The pseudo groups 0 (rows before the first group) and
-// groups + 1 (behind the last) take part. Every thread of the workgroup calls.
-// Where the offsets decrease somewhere, groups overlap or miss rows, but every
-// tile still lies in [0, rows), and there are no more of them than the grid has.
+// The number of row tiles of BP rows, and which rows the tile `index` of them holds.
+// A thread has a run of groups, and knows how many tiles come before them. The pseudo
+// groups 0 (rows before the first group) and groups + 1 (behind the last) take part. Every
+// thread of the workgroup calls. Where the offsets decrease somewhere, groups overlap or
+// miss rows, but every tile still lies in [0, rows), and there are no more of them than
+// the grid has room for.
 template <int BP, int THREADS>
 struct RowTiles {
-  static constexpr int kPer = (kMaxGroups + 2 + THREADS - 1) / THREADS;
-  int first[kPer];  // tiles before this thread's groups
-  int64_t lo[kPer];
-  int n[kPer];
-  int total;
+  struct Shared {
+    int bound[kMaxGroups + 1];  // the offsets, in [0, rows]
+    int sums[THREADS / 64];     // tiles of each wave's groups
+    int found[3];               // a tile: its first row, its rows, its group
+  };
+  Shared& in;
+  int groups, rows, per, first, total;
 
-  // slots: THREADS / 64 ints; found: 2 words. `most`: tiles that the grid has room for.
-  __device__ RowTiles(const int64_t* offsets, int groups, int64_t rows, int most, int* slots, int64_t* found) {
+  // `most`: tiles that the grid has room for.
+  __device__ RowTiles(Shared& shared, const int64_t* offsets, int groups_, int64_t rows_, int most)
+      : in(shared), groups(groups_), rows((int)rows_), per((groups_ + 1 + THREADS) / THREADS) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid < 2) found[tid] = 0;
-    const int per = (groups + 2 + THREADS - 1) / THREADS;
+    for (int e = tid; e <= groups; e += THREADS) in.bound[e] = (int)clamp_row(offsets[e], rows);
+    if (tid < 3) in.found[tid] = 0;  // for a tile past the last one
+    __syncthreads();
     int sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = tid * per + i;
-      lo[i] = 0;
-      n[i] = 0;
-      if (i < per && e < groups + 2) {
-        lo[i] = e == 0 ? 0 : clamp_row(offsets[e - 1], rows);
-        const int64_t hi = e == groups + 1 ? rows : clamp_row(offsets[e], rows);
-        n[i] = hi > lo[i] ? (int)(hi - lo[i]) : 0;
-      }
-      first[i] = sum;
-      sum += (n[i] + BP - 1) / BP;
-    }
+    for (int i = 0; i < per; ++i) sum += count(tid * per + i);
     int before = sum;  // inclusive prefix over the wave
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const int v = __shfl_up(before, d);
       if (lane >= d) before += v;
     }
-    if (lane == 63) slots[wave] = before;
+    if (lane == 63) in.sums[wave] = before;
     __syncthreads();
-    int base = before - sum;
+    first = before - sum;
     total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 64; ++w) {
-      const int v = slots[w];
-      if (w < wave) base += v;
+      const int v = in.sums[w];
+      if (w < wave) first += v;
       total += v;
     }
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) first[i] += base;
-    total = total < 0 || total > most ? most : total;
+    total = __builtin_amdgcn_readfirstlane(total < 0 || total > most ? most : total);
   }
+  __device__ int begin(int e) const { return e == 0 ? 0 : in.bound[e - 1]; }
+  __device__ int height(int e) const {
+    if (e > groups + 1) return 0;
+    const int n = (e == groups + 1 ? rows : in.bound[e]) - begin(e);
+    return n > 0 ? n : 0;
+  }
+  __device__ int count(int e) const { return (height(e) + BP - 1) / BP; }
 
-  __device__ RowTileAt at(int index, int groups, int64_t* found) const {
-    const int tid = threadIdx.x;
-    const int per = (groups + 2 + THREADS - 1) / THREADS;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int k = index - first[i];
-      if (k >= 0 && k < (n[i] + BP - 1) / BP) {
-        const int e = tid * per + i;
-        found[0] = lo[i] + (int64_t)k * BP;
-        found[1] = ((int64_t)(n[i] - k * BP < BP ? n[i] - k * BP : BP) << 32) | (uint32_t)(e == groups + 1 ? 0 : e);
+  __device__ RowTileAt at(int index) const {
+    int before = first;
+    for (int i = 0; i < per; ++i) {
+      const int e = (int)threadIdx.x * per + i, n = height(e), k = index - before;
+      before += (n + BP - 1) / BP;
+      if (k >= 0 && index < before) {
+        in.found[0] = begin(e) + k * BP;
+        in.found[1] = n - k * BP < BP ? n - k * BP : BP;
+        in.found[2] = e == groups + 1 ? 0 : e;
       }
     }
     __syncthreads();
-    const int64_t row = found[0], w = found[1];
     RowTileAt t;
-    t.row = uniform(row);
-    t.count = __builtin_amdgcn_readfirstlane((int)(w >> 32));
-    t.group = __builtin_amdgcn_readfirstlane((int)(uint32_t)w) - 1;
+    t.row = __builtin_amdgcn_readfirstlane(in.found[0]);
+    t.count = __builtin_amdgcn_readfirstlane(in.found[1]);
+    t.group = __builtin_amdgcn_readfirstlane(in.found[2]) - 1;
     return t;
   }
-
 };
 
 // Workgroups go to the 8 XCDs in turn; this numbering gives each XCD one run of
@@ -472,7 +466,10 @@ struct ColOperand {
 
   // Load i straight into LDS; rows past the last and chunks past the tile's columns as zeros.
   __device__ static void place(LdsPtr lds, int i) { lds_place(lds + (i * NW + wave_of<NW>()) * 1024); }
-  __device__ void fetch(int i) const { load_to_place<16, false>(buffer_from(base), off[i]); }
+  template <bool ONCE = false>
+  __device__ void fetch(int i) const {
+    load_to_place<16, ONCE>(buffer_from(base), off[i]);
+  }
   // A row past the last is the last; what a chunk holds past the tile's columns does
   // not matter, since nothing of it is stored.
   __device__ void load(u32x4 (&v)[kLoads]) const {
@@ -650,7 +647,8 @@ struct Folded {
   }
 };
 
-template <class T, class P, class Q, class PS, class QS, int WP, int WQ, int FP, int FQ, int STEP>
+// ONCE: Q's loads as of data that no other workgroup reads.
+template <class T, class P, class Q, class PS, class QS, int WP, int WQ, int FP, int FQ, int STEP, bool ONCE = false>
 struct Product {
   static constexpr bool kDirect = STEP == 128;  // straight into LDS, or (64) through registers
   static constexpr int kSlots = kDirect ? 2 : 4;
@@ -797,7 +795,7 @@ struct Product {
       if (i < kP) {
         p.fetch(i);
       } else if (i < kQ) {
-        q.fetch(i - kP);
+        q.template fetch<ONCE>(i - kP);
       } else if (i < kPS) {
         ps.fetch(i - kQ);
       } else {
@@ -960,7 +958,8 @@ __device__ inline void store_zeros(char* out, int64_t ld, int rows, int cols) {
 // rows, which cost 18000 cycles for a tile of 256 x 256: a third of a weight gradient of
 // 1024 rows an expert (1006 us, against 705 with an eighth of the stores). So the wave
 // turns its part over in `lds`, SPACE bytes that it keeps to itself: stores take whole
-// rows of it. Vectors are stored at any byte.
+// rows of it, past the caches (64 experts of 96 rows, 1408 x 2048: weight gradient 108 us,
+// 144 through them). Vectors are stored at any byte.
 template <class C, bool PERM, int FP, int FQ, int SPACE>
 __device__ inline void store_tile(const f32x4 (&acc)[FP][FQ], LdsPtr lds, char* out, int64_t ld, int p0, int q0,
                                   int rows, int cols) {
@@ -1004,7 +1003,7 @@ __device__ inline void store_tile(const f32x4 (&acc)[FP][FQ], LdsPtr lds, char* 
       char* const to = out + ((int64_t)p * ld + q) * C::kBytes;
       if (p < rows) {
         if (q + C::VEC <= cols) {
-          *reinterpret_cast<u32x4_any*>(to) = w;
+          __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(to));
         } else if (q < cols) {
           store_partial<C>(w, cols - q, to);
         }
@@ -1050,7 +1049,7 @@ struct RowsArgs {
 // (256 a lane) for 16. 64, and tiles that go through registers, need more.
 constexpr int tile_waves(int fragments, bool direct) { return direct && fragments <= 16 ? 2 : 1; }
 
-template <class T, class C, bool QROWS, int WP, int WQ, int FP, int FQ, bool DIRECT>
+template <class T, class C, bool QROWS, int WP, int WQ, int FP, int FQ, bool DIRECT, bool ONCE>
 __global__ __launch_bounds__(WP* WQ * 64, tile_waves(FP* FQ, DIRECT)) void rows_product(RowsArgs a) {
   constexpr int BP = WP * FP * 16, BQ = WQ * FQ * 16, NW = WP * WQ, kStep = DIRECT ? 128 : 64;
   using P = RowOperand<T, BP, NW, false, kStep>;
@@ -1058,19 +1057,18 @@ __global__ __launch_bounds__(WP* WQ * 64, tile_waves(FP* FQ, DIRECT)) void rows_
   using Q = std::conditional_t<QROWS, RowOperand<T, BQ, NW, kPerm, kStep>, ColOperand<T, BQ, NW, kStep>>;
   using PS = std::conditional_t<T::kScaled, Scales<P, BP, NW, FP, kStep>, NoScales>;
   using QS = std::conditional_t<T::kScaled, Scales<Q, BQ, NW, FQ, kStep>, NoScales>;
-  using Prod = Product<T, P, Q, PS, QS, WP, WQ, FP, FQ, kStep>;
+  using Prod = Product<T, P, Q, PS, QS, WP, WQ, FP, FQ, kStep, ONCE>;
   __shared__ __attribute__((aligned(1024))) char lds[Prod::kLds];
-  __shared__ int slots[NW];
-  __shared__ int64_t found[2];
+  __shared__ typename RowTiles<BP, NW * 64>::Shared shared;
 
   RowTileAt at;
   int tp, tq;
   if (a.offsets != nullptr) {
-    const RowTiles<BP, NW * 64> tiles(a.offsets, a.groups, a.rows, a.most, slots, found);
+    const RowTiles<BP, NW * 64> tiles(shared, a.offsets, a.groups, a.rows, a.most);
     const int total = tiles.total * a.tiles_q;
     if ((int)blockIdx.x >= total) return;
     tile_order(xcd_contiguous(blockIdx.x, total), tiles.total, a.tiles_q, &tp, &tq);
-    at = tiles.at(tp, a.groups, found);
+    at = tiles.at(tp);
     if (at.count == 0) return;
   } else {
     tile_order(xcd_contiguous(blockIdx.x, gridDim.x), a.most, a.tiles_q, &tp, &tq);
@@ -1301,17 +1299,16 @@ __global__ __launch_bounds__(NW * 64, DEPTH ? 1 : 2) void rows_stream(RowsArgs a
   using Ring = StreamRing<T, FP, FQ, NW, DEPTH>;
   constexpr int kSums = NW * FP * FQ * 1024;
   __shared__ __attribute__((aligned(1024))) char lds[NW * Ring::kLds > kSums ? NW * Ring::kLds : kSums];
-  __shared__ int slots[NW];
-  __shared__ int64_t found[2];
+  __shared__ typename RowTiles<BP, NW * 64>::Shared shared;
 
   RowTileAt at;
   int tp, tq;
   if (a.offsets != nullptr) {
-    const RowTiles<BP, NW * 64> tiles(a.offsets, a.groups, a.rows, a.most, slots, found);
+    const RowTiles<BP, NW * 64> tiles(shared, a.offsets, a.groups, a.rows, a.most);
     const int total = tiles.total * a.tiles_q;
     if ((int)blockIdx.x >= total) return;
     tile_order(xcd_contiguous(blockIdx.x, total), tiles.total, a.tiles_q, &tp, &tq);
-    at = tiles.at(tp, a.groups, found);
+    at = tiles.at(tp);
     if (at.count == 0) return;
   } else {
     tile_order(xcd_contiguous(blockIdx.x, gridDim.x), a.most, a.tiles_q, &tp, &tq);
@@ -1429,9 +1426,9 @@ int32_t launch_rows_grid(void (*kernel)(RowsArgs), int threads, RowsArgs a, hipS
   return launch_status();
 }
 
-template <class T, class C, bool QROWS, int WP, int WQ, int FP, int FQ, bool DIRECT>
+template <class T, class C, bool QROWS, int WP, int WQ, int FP, int FQ, bool DIRECT, bool ONCE = false>
 int32_t launch_rows(const RowsArgs& a, hipStream_t st) {
-  return launch_rows_grid<WP * FP * 16, WQ * FQ * 16>(rows_product<T, C, QROWS, WP, WQ, FP, FQ, DIRECT>,
+  return launch_rows_grid<WP * FP * 16, WQ * FQ * 16>(rows_product<T, C, QROWS, WP, WQ, FP, FQ, DIRECT, ONCE>,
                                                       WP * WQ * 64, a, st);
 }
 
@@ -1440,10 +1437,17 @@ int32_t launch_stream(const RowsArgs& a, hipStream_t st) {
   return launch_rows_grid<FP * 16, FQ * 16>(rows_stream<T, C, FP, FQ, NW, DEPTH>, NW * 64, a, st);
 }
 
-// Tiles of 256 x 256 pay where they are filled, and enough to give each of the 256 CUs one:
-// groups of `filled` rows on average, and as many tiles (one cut short a group).
-inline bool wide_tiles(const RowsArgs& a, int64_t filled) {
-  return a.rows >= filled * a.groups && (a.rows / 256 + a.groups / 2) * ((a.cols + 255) / 256) >= 200;
+// Tiles of 256 x 256, of which a SIMD's one wave reads a quarter less from LDS for a
+// product, pay where they are filled and enough for the 256 CUs (one cut short a group).
+// bf16, us, forward and input gradient, against 128 x 128: 8 groups of 1024 rows, 14336 x
+// 4096 781 and 882 (128 x 128: 1057 and 1138); of 128 rows 196 and 279 (238 and 296), of 64
+// rows 207 and 242 (187 and 197); 64 groups of 128 rows, 1408 x 2048 116 and 115 (105 and
+// 102), of 256 rows 159 and 121 (166 and 156); 8 of 512 rows, 2048 x 2048, 160 tiles, 49 and
+// 50 (68 and 64), 2048 rows, 4096 x 4096, 128 tiles, 81 and 82 (69 and 73).
+template <class T>
+inline bool wide_tiles(const RowsArgs& a) {
+  return T::kAccumulates && a.rows >= 128 * (int64_t)a.groups &&
+         (a.rows / 256 + a.groups / 2) * ((a.cols + 255) / 256) >= 150;
 }
 
 // Tiles of 128 x 128, or of 64 x 64 where there would be fewer than 192 of those for the
@@ -1455,6 +1459,11 @@ template <class T, class C, bool QROWS, bool WHOLE>
 int32_t launch_rows_small(const RowsArgs& a, hipStream_t st) {
   if constexpr (T::kBytes != 4) {
     if ((a.rows / 128 + a.groups / 2 + 1) * ((a.cols + 127) / 128) >= 192) {
+      // Groups that fill one tile on average: their weights are read once, past the caches (160
+      // groups of 77 rows, 1536 x 2048: 212 us against 220; of 200 rows 133 against 131).
+      if constexpr (WHOLE) {
+        if (a.rows <= 96 * (int64_t)a.groups) return launch_rows<T, C, QROWS, 2, 2, 4, 4, true, true>(a, st);
+      }
       return launch_rows<T, C, QROWS, 2, 2, 4, 4, WHOLE>(a, st);
     }
   }
@@ -1473,7 +1482,7 @@ int32_t launch_rows_by_size(const RowsArgs& a, hipStream_t st) {
     return WHOLE ? launch_stream<T, C, 4, 4, 4, 2>(a, st) : launch_stream<T, C, 2, 2, 4, 0>(a, st);
   }
   if constexpr (WHOLE && T::kAccumulates) {
-    if (wide_tiles(a, 128)) return launch_rows<T, C, true, 2, 2, 8, 8, true>(a, st);
+    if (wide_tiles<T>(a)) return launch_rows<T, C, true, 2, 2, 8, 8, true>(a, st);
   }
   return launch_rows_small<T, C, true, WHOLE>(a, st);
 }

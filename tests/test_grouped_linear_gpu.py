@@ -269,7 +269,7 @@ def test_large_tiles_grad_weight(n, k, dtype):
     """Experts of 0 to 1000 rows; weights in full and cut tiles, and of few rows or columns."""
     sizes = [1000, 1, 0, 129, 256] if n * k < 1 << 20 else [520, 0, 330]
     offsets = _offsets(sizes, 2)
-    rows = max(int(offsets[-1]) + 5, 256 * len(sizes))
+    rows = max(int(offsets[-1]) + 5, 768 * len(sizes))
     g, x = _ints((rows, n), 4, dtype, n), _ints((rows, k), 4, dtype, k)
     got = K.grouped_linear_grad_weight(g.cuda(), x.cuda(), offsets.cuda()).cpu()
     want = _rounded(products.grouped_linear_grad_weight(_np(g), _np(x), offsets.numpy()), dtype)
