@@ -226,14 +226,13 @@ __device__ inline int xcd_contiguous(int id, int total) {
   return xcd * each + (xcd < rest ? xcd : rest) + k;
 }
 
-// Tiles in blocks of kBlockP row tiles, in each block the row tiles of one
-// column tile after another: what runs at the same time on an XCD shares rows
-// of P and of Q.
-constexpr int kBlockP = 8;
+// Tiles in blocks of HEIGHT row tiles, in each block the row tiles of one column tile
+// after another: what runs at the same time on an XCD shares rows of P and of Q.
+template <int HEIGHT = 8>
 __device__ inline void tile_order(int t, int tiles_p, int tiles_q, int* tp, int* tq) {
-  const int block = t / (kBlockP * tiles_q), p0 = block * kBlockP;
-  const int height = tiles_p - p0 < kBlockP ? tiles_p - p0 : kBlockP;
-  const int r = t - block * kBlockP * tiles_q;
+  const int block = t / (HEIGHT * tiles_q), p0 = block * HEIGHT;
+  const int height = tiles_p - p0 < HEIGHT ? tiles_p - p0 : HEIGHT;
+  const int r = t - block * HEIGHT * tiles_q;
   *tq = r / height;
   *tp = p0 + r % height;
 }
@@ -950,7 +949,17 @@ __device__ inline S scales_of(const char* p, int64_t blocks, int rows) {
 // Zeros in the workgroup's tile of NW waves: `rows` rows of `cols` columns.
 template <class C, int NW>
 __device__ inline void store_zeros(char* out, int64_t ld, int rows, int cols) {
-  for (int i = threadIdx.x; i < rows * cols; i += NW * 64) C::store1(out, (int64_t)(i / cols) * ld + i % cols, 0.0f);
+  const u32x4 zeros = {0u, 0u, 0u, 0u};
+  const int chunks = (cols + C::VEC - 1) / C::VEC;
+  for (int i = threadIdx.x; i < rows * chunks; i += NW * 64) {
+    const int row = i / chunks, q = (i - row * chunks) * C::VEC;
+    char* const to = out + ((int64_t)row * ld + q) * C::kBytes;
+    if (q + C::VEC <= cols) {
+      __builtin_nontemporal_store(zeros, reinterpret_cast<u32x4_any*>(to));
+    } else {
+      store_partial<C>(zeros, cols - q, to);
+    }
+  }
 }
 
 // Stores a wave's fragments: rows [p0, rows) of `out` (row stride ld elements), columns
@@ -1061,17 +1070,19 @@ __global__ __launch_bounds__(WP* WQ * 64, tile_waves(FP* FQ, DIRECT)) void rows_
   __shared__ __attribute__((aligned(1024))) char lds[Prod::kLds];
   __shared__ typename RowTiles<BP, NW * 64>::Shared shared;
 
+  // Row tiles that mostly are of groups apart share no weights: one group's are read in one run.
+  constexpr int kHeight = ONCE ? 2 : 8;
   RowTileAt at;
   int tp, tq;
   if (a.offsets != nullptr) {
     const RowTiles<BP, NW * 64> tiles(shared, a.offsets, a.groups, a.rows, a.most);
     const int total = tiles.total * a.tiles_q;
     if ((int)blockIdx.x >= total) return;
-    tile_order(xcd_contiguous(blockIdx.x, total), tiles.total, a.tiles_q, &tp, &tq);
+    tile_order<kHeight>(xcd_contiguous(blockIdx.x, total), tiles.total, a.tiles_q, &tp, &tq);
     at = tiles.at(tp);
     if (at.count == 0) return;
   } else {
-    tile_order(xcd_contiguous(blockIdx.x, gridDim.x), a.most, a.tiles_q, &tp, &tq);
+    tile_order<kHeight>(xcd_contiguous(blockIdx.x, gridDim.x), a.most, a.tiles_q, &tp, &tq);
     at.row = (int64_t)tp * BP;
     at.count = a.rows - at.row < BP ? (int)(a.rows - at.row) : BP;
     at.group = 0;
@@ -1459,8 +1470,9 @@ template <class T, class C, bool QROWS, bool WHOLE>
 int32_t launch_rows_small(const RowsArgs& a, hipStream_t st) {
   if constexpr (T::kBytes != 4) {
     if ((a.rows / 128 + a.groups / 2 + 1) * ((a.cols + 127) / 128) >= 192) {
-      // Groups that fill one tile on average: their weights are read once, past the caches (160
-      // groups of 77 rows, 1536 x 2048: 212 us against 220; of 200 rows 133 against 131).
+      // Groups that fill one tile on average: their weights are read once, past the caches and
+      // group after group (160 groups of 77 rows, 1536 x 2048: 212 us against 220 through the
+      // caches, 5 of them for the order; 64 groups of 200 rows, 1408 x 2048: 133 against 131).
       if constexpr (WHOLE) {
         if (a.rows <= 96 * (int64_t)a.groups) return launch_rows<T, C, QROWS, 2, 2, 4, 4, true, true>(a, st);
       }
