@@ -86,10 +86,9 @@ struct ElemF16 {
                                                   0);
   }
 };
-// Four MFMAs of depth 4: MFMA j takes element j of every lane's chunk. Sums are
-// folded every 16 halves of steps (256 elements) into a second accumulator, so that their
-// rounding errors do not grow with the whole length: 10000 normal products are off
-// by a third of what one running sum is off by.
+// Four MFMAs of depth 4: MFMA j takes element j of every lane's chunk. Sums are folded
+// every 16 halves of steps (256 elements) into a second accumulator, so that their rounding
+// errors do not grow with the whole length.
 struct ElemF32 {
   static constexpr bool kAccumulates = false;
   static constexpr int kFold = 16;
@@ -172,7 +171,7 @@ struct RowTiles {
     if (tid < 3) in.found[tid] = 0;  // for a tile past the last one
     __syncthreads();
     int sum = 0;
-    for (int i = 0; i < per; ++i) sum += count(tid * per + i);
+    for (int i = 0; i < per; ++i) sum += tiles_of(height(tid * per + i));
     int before = sum;  // inclusive prefix over the wave
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -197,13 +196,13 @@ struct RowTiles {
     const int n = (e == groups + 1 ? rows : in.bound[e]) - begin(e);
     return n > 0 ? n : 0;
   }
-  __device__ int count(int e) const { return (height(e) + BP - 1) / BP; }
+  __device__ static int tiles_of(int n) { return (int)(((uint32_t)n + BP - 1) / BP); }
 
   __device__ RowTileAt at(int index) const {
     int before = first;
     for (int i = 0; i < per; ++i) {
       const int e = (int)threadIdx.x * per + i, n = height(e), k = index - before;
-      before += (n + BP - 1) / BP;
+      before += tiles_of(n);
       if (k >= 0 && index < before) {
         in.found[0] = begin(e) + k * BP;
         in.found[1] = n - k * BP < BP ? n - k * BP : BP;
@@ -213,7 +212,9 @@ struct RowTiles {
     __syncthreads();
     RowTileAt t;
     t.row = __builtin_amdgcn_readfirstlane(in.found[0]);
-    t.count = __builtin_amdgcn_readfirstlane(in.found[1]);
+    // Offsets in no order can name a tile twice: still none of it past the last row.
+    const int count = __builtin_amdgcn_readfirstlane(in.found[1]), left = rows - (int)t.row;
+    t.count = count < left ? count : left;
     t.group = __builtin_amdgcn_readfirstlane(in.found[2]) - 1;
     return t;
   }
@@ -1466,10 +1467,14 @@ inline bool wide_tiles(const RowsArgs& a) {
 // against 28.4; 16 of 128, 2048 x 1024, 200 tiles 32.9 against 34.7), and always for fp32,
 // whose products take the matrix cores 16 times as long (13 groups of 77 rows, 1003 x 777:
 // 70.6 against 40.7; 4096 rows, 4096 x 4096: 955 against 980).
+template <class T>
+inline bool middle_tiles(const RowsArgs& a) {
+  return T::kBytes != 4 && (a.rows / 128 + a.groups / 2 + 1) * ((a.cols + 127) / 128) >= 192;
+}
 template <class T, class C, bool QROWS, bool WHOLE>
 int32_t launch_rows_small(const RowsArgs& a, hipStream_t st) {
   if constexpr (T::kBytes != 4) {
-    if ((a.rows / 128 + a.groups / 2 + 1) * ((a.cols + 127) / 128) >= 192) {
+    if (middle_tiles<T>(a)) {
       // Groups that fill one tile on average: their weights are read once, past the caches and
       // group after group (160 groups of 77 rows, 1536 x 2048: 212 us against 220 through the
       // caches, 5 of them for the order; 64 groups of 200 rows, 1408 x 2048: 133 against 131).
@@ -1482,16 +1487,25 @@ int32_t launch_rows_small(const RowsArgs& a, hipStream_t st) {
   return launch_rows<T, C, QROWS, 2, 2, 2, 2, WHOLE>(a, st);
 }
 
-// Which kernel, for weights that are rows of the contracted index.
+// Which kernel, for weights that are rows of the contracted index. The streams of few rows read
+// the weights once for each 16 or 32 rows, so they are for groups that mostly have no more:
+// up to half of that on average, or all of it if there is one group; and the longer one also
+// where tiles are few. bf16, us, streams of 16 rows, of 32, and 128 x 128 tiles: 8 groups of 2
+// rows, 14336 x 4096 121, 123, 149, of 8 rows 150, 153, 163, of 16 rows 208, 171, 152, of 32
+// rows 315, 243, 158; 64 groups of 8 rows, 1408 x 2048 60, 70, 85, of 16 rows 77, 75, 83, of 24
+// rows 97, 84, 84; one of 32 rows, 4096 x 4096 11, 14, 49, 14336 x 4096 33, 26, 51. Two fragments
+// of columns a workgroup, or one where that leaves CUs without (one group of 8 rows,
+// 4096 x 4096 10.7 and 9.8; 64 of 8, 1408 x 2048 60 and 65).
 template <class T, class C, bool WHOLE>
 int32_t launch_rows_by_size(const RowsArgs& a, hipStream_t st) {
-  if (a.rows <= 16 * (int64_t)a.groups) {
+  const bool one = a.groups == 1;
+  if (a.rows <= (one ? 16 : 8) * (int64_t)a.groups) {
     const int64_t tiles = a.rows < a.groups ? a.rows : a.groups;
     if (tiles * a.cols >= 256 * 32) return launch_stream<T, C, 1, 2, 4, WHOLE ? 2 : 0>(a, st);
     return launch_stream<T, C, 1, 1, 4, WHOLE ? 2 : 0>(a, st);
   }
-  if (a.rows <= 32 * (int64_t)a.groups) {
-    return WHOLE ? launch_stream<T, C, 4, 4, 4, 2>(a, st) : launch_stream<T, C, 2, 2, 4, 0>(a, st);
+  if (a.rows <= (one || !middle_tiles<T>(a) ? 32 : 16) * (int64_t)a.groups) {
+    return launch_stream<T, C, 2, 2, 4, WHOLE ? 2 : 0>(a, st);
   }
   if constexpr (WHOLE && T::kAccumulates) {
     if (wide_tiles<T>(a)) return launch_rows<T, C, true, 2, 2, 8, 8, true>(a, st);

@@ -276,13 +276,16 @@ def test_large_tiles_grad_weight(n, k, dtype):
     assert torch.equal(got, want), (got != want).nonzero()[:4].tolist()
 
 
-@pytest.mark.parametrize("per", [1, 8, 16, 17, 32, 33, 64, 127, 129])
+@pytest.mark.parametrize("per", [1, 8, 9, 16, 17, 32, 33, 64, 127, 129])
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_rows_a_group(per, dtype):
     """Either side of the average group sizes that other kernels take, with uneven groups."""
     sizes = [0, 2 * per, per, per + 1, per - 1]
     _check_ints(sizes, 200, 264, dtype, seed=per)
     _check_ints(sizes, 67, 75, dtype, seed=per)
+    _check_ints([per], 100, 136, dtype, seed=per)
+    if per in (16, 32, 33):  # with tiles enough
+        _check_ints(sizes, 8200, 72, dtype, seed=per)
 
 
 def test_large_tiles_twice_alike():

@@ -227,5 +227,7 @@ def test_large_tiles_dense():
 @pytest.mark.parametrize("per", [1, 16, 17, 32, 33, 127, 129])
 def test_rows_a_group(per):
     """Either side of the average group sizes that other kernels take, with uneven groups."""
+    _check_linear([0, 2 * per, per, per + 1, per - 1], 8200, 128, torch.bfloat16, seed=per, low=126, high=128)
     for k in (256, 224):
+        _check_linear([per], 150, k, torch.bfloat16, seed=per, dense=True, low=126, high=128)
         _check_linear([0, 2 * per, per, per + 1, per - 1], 150, k, torch.bfloat16, seed=per, low=126, high=128)
