@@ -704,6 +704,9 @@ struct Product {
 
   // Half a step's products are issued in kParts parts, with reads and loads between them:
   // one by one where a SIMD has a single wave to issue anything (kWide), else by rows.
+  // 256 x 256 tiles take 2250 cycles a step so, of which the matrix cores need 2048 (8192 rows
+  // on 8 groups of 14336 x 4096, bf16: 786 us, 1.22 PFLOP/s; 128 x 128 tiles, two workgroups a
+  // CU, which LDS bounds, 1057).
   static constexpr bool kWide = FP == 8 && FQ == 8;
   // Sums in the accumulation registers: for the wide ones, and for the scaled products, whose
   // builtin takes operands of twice the size, zeros behind what there is of them.
@@ -964,12 +967,11 @@ __device__ inline void store_zeros(char* out, int64_t ld, int rows, int cols) {
 }
 
 // Stores a wave's fragments: rows [p0, rows) of `out` (row stride ld elements), columns
-// [q0, cols). Straight from the registers a store takes 16 or 8 bytes of each of 16
-// rows, which cost 18000 cycles for a tile of 256 x 256: a third of a weight gradient of
-// 1024 rows an expert (1006 us, against 705 with an eighth of the stores). So the wave
-// turns its part over in `lds`, SPACE bytes that it keeps to itself: stores take whole
-// rows of it, past the caches (64 experts of 96 rows, 1408 x 2048: weight gradient 108 us,
-// 144 through them). Vectors are stored at any byte.
+// [q0, cols). Straight from the registers a store would take 16 or 8 bytes of each of 16
+// rows. So the wave turns its part over in `lds`, SPACE bytes that it keeps to itself, and
+// stores take whole rows of it (weight gradient of 8192 rows, 8 experts of 14336 x 4096: 937
+// us, 1006 straight), past the caches (64 experts of 96 rows, 1408 x 2048: 108 us, 144
+// through them). Vectors are stored at any byte.
 template <class C, bool PERM, int FP, int FQ, int SPACE>
 __device__ inline void store_tile(const f32x4 (&acc)[FP][FQ], LdsPtr lds, char* out, int64_t ld, int p0, int q0,
                                   int rows, int cols) {
@@ -1117,7 +1119,10 @@ __global__ __launch_bounds__(WP* WQ * 64, tile_waves(FP* FQ, DIRECT)) void rows_
 // ---------------------------------------------------------------------------
 // Few rows a group: the weights are read once, and that is the time. A workgroup
 // owns FP x 16 rows and FQ x 16 columns; its NW waves take the contracted index in
-// turn, and their sums meet in LDS at the end, in the order of the waves.
+// turn, and their sums meet in LDS at the end, in the order of the waves. 16 rows on 8
+// groups of 14336 x 4096, bf16: 118 us, 7.1 TB/s; straight from memory to registers, as
+// rows off their alignment take, 160 to 200. A ring of two steps was as good as any deeper
+// one, and 32 columns a workgroup of four waves as good as other shapes.
 // ---------------------------------------------------------------------------
 
 constexpr int kStreamBytes = 256, kStreamSteps = kStreamBytes / 64;
