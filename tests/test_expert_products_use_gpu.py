@@ -247,3 +247,34 @@ def test_mxfp4_past_2_31_elements():
     xv, wv = K.mxfp4_dequant(*few, k, torch.float32).abs().double(), K.mxfp4_dequant(*w, k, torch.float32).abs().double()
     bound = 2 * (k + 2) * 2.0 ** -24 * (xv @ wv.T) + 2.0 ** -7 * one.abs()
     assert ((y[at].double() - one).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("op", ["grouped_linear", "mxfp4"])
+def test_cli_targets(op):
+    """What `compare` and `profile` call: kernel and formula agree up to the formula's own roundings (bf16 products'
+    sums and results, so a step of 2^-7 of the largest magnitude covers both)."""
+    from custom_cuda_kernals_amd.cli.registry import REGISTRY
+
+    target = REGISTRY[op].build_target("cuda")
+    got, want = target.kernel().double(), target.eager().double()
+    assert got.shape == want.shape
+    assert (got - want).abs().max() <= 2.0 ** -7 * want.abs().max()
+
+
+@pytest.mark.parametrize("groups", [1024, 1000])
+def test_offsets_in_no_order_of_many_groups(groups):
+    """As many groups as are taken, each of them as long as the rows or of none in turn: every tile named is inside,
+    and the calls end; nothing behind the outputs is written."""
+    rows, n, k = 5000, 64, 64
+    o = torch.zeros(groups + 1, dtype=torch.int64)
+    o[1::2] = rows
+    o = o.cuda()
+    buffers = [torch.full((size + 4096,), 55, dtype=torch.bfloat16, device="cuda")
+               for size in (rows * n, rows * k, groups * n * k)]
+    x, g, w = _randn(rows, k, seed=1), _randn(rows, n, seed=2), _randn(groups, n, k, seed=3)
+    native.grouped_linear_fwd(x, w, o, buffers[0][:rows * n].view(rows, n))
+    native.grouped_linear_grad_input(g, w, o, buffers[1][:rows * k].view(rows, k))
+    native.grouped_linear_grad_weight(g, x, o, buffers[2][:groups * n * k].view(groups, n, k))
+    torch.cuda.synchronize()
+    for b in buffers:
+        assert (b[-4096:] == 55).all()
