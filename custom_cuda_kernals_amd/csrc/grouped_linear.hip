@@ -29,7 +29,7 @@ __host__ __device__ constexpr int weights_room(int each) { return each < kTilesA
 template <class T, class C, int WP, int WQ, int FP, int FQ, bool DIRECT>
 __global__ __launch_bounds__(WP* WQ * 64, tile_waves(FP* FQ, DIRECT)) void grouped_weights(
     const char* __restrict__ grad, const char* __restrict__ x, const int64_t* __restrict__ offsets,
-    char* __restrict__ out, int64_t rows, int n, int k, int tiles_p, int tiles_q) {
+    char* __restrict__ out, int64_t rows, int n, int k, int tiles_p, int tiles_q, int first, int total) {
   constexpr int BP = WP * FP * 16, BQ = WQ * FQ * 16, NW = WP * WQ, kStep = DIRECT ? 128 : 64;
   using P = ColOperand<T, BP, NW, kStep>;
   using Q = ColOperand<T, BQ, NW, kStep>;
@@ -37,13 +37,14 @@ __global__ __launch_bounds__(WP* WQ * 64, tile_waves(FP* FQ, DIRECT)) void group
   __shared__ __attribute__((aligned(1024))) char lds[Prod::kLds];
 
   const int each = tiles_p * tiles_q, room = weights_room(each);
+  const int id = first + (int)blockIdx.x;
   int e, t;
   if (room >= kTilesApart) {
-    e = blockIdx.x / room;
-    t = xcd_contiguous(blockIdx.x - e * room, room);
+    e = id / room;
+    t = xcd_contiguous(id - e * room, room);
     if (t >= each) return;
   } else {
-    t = xcd_contiguous(blockIdx.x, gridDim.x);
+    t = xcd_contiguous(id, total);
     e = t / each;
     t -= e * each;
   }
@@ -97,7 +98,7 @@ int32_t grouped_rows(const void* x, const void* w, const int64_t* offsets, void*
     if (rows <= 0 || length <= 0 || cols <= 0) return (int32_t)hipSuccess;
     if (!sizes_ok(rows, groups, cols * T::kBytes, length * T::kBytes)) return (int32_t)hipErrorInvalidValue;
     const RowsArgs a = {static_cast<const char*>(x), static_cast<const char*>(w), nullptr, nullptr, offsets,
-                        static_cast<char*>(out), rows, length, (int)groups, (int)cols, 0, 0};
+                        static_cast<char*>(out), rows, length, (int)groups, (int)cols, 0, 0, 0};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (length * T::kBytes < 16 || (!QROWS && cols * T::kBytes < 16)) {
       const NarrowArgs n = {a.x, a.w, offsets, a.out, rows, length, 1, QROWS ? length : 1, QROWS ? 1 : cols,
@@ -122,13 +123,13 @@ int32_t run_weights(const void* grad, const void* x, const int64_t* offsets, voi
                     int64_t n, int64_t k, hipStream_t st) {
   constexpr int BP = WP * FP * 16, BQ = WQ * FQ * 16, NW = WP * WQ;
   const int64_t tiles_p = (n + BP - 1) / BP, tiles_q = (k + BQ - 1) / BQ;
-  if (groups * (tiles_p * tiles_q + 7) * NW * 64 >= kMaxThreads) return (int32_t)hipErrorInvalidValue;
-  const int64_t grid = groups * weights_room((int)(tiles_p * tiles_q));
-  grouped_weights<T, C, WP, WQ, FP, FQ, DIRECT>
-      <<<(unsigned)grid, NW * 64, 0, st>>>(
-          static_cast<const char*>(grad), static_cast<const char*>(x), offsets, static_cast<char*>(out), rows, (int)n,
-          (int)k, (int)tiles_p, (int)tiles_q);
-  return launch_status();
+  if (tiles_p * tiles_q > INT32_MAX - 7) return (int32_t)hipErrorInvalidValue;
+  const int64_t total = groups * weights_room((int)(tiles_p * tiles_q));
+  return launch_tiles(total, NW * 64, [&](int first, unsigned count) {
+    grouped_weights<T, C, WP, WQ, FP, FQ, DIRECT><<<count, NW * 64, 0, st>>>(
+        static_cast<const char*>(grad), static_cast<const char*>(x), offsets, static_cast<char*>(out), rows, (int)n,
+        (int)k, (int)tiles_p, (int)tiles_q, first, (int)total);
+  });
 }
 
 // Tiles of 256 x 256 where experts have 768 rows or more on average and each CU gets a tile

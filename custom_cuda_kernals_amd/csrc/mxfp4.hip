@@ -212,7 +212,7 @@ extern "C" int32_t launch_mxfp4_linear_fwd(const void* x_codes, const void* x_sc
     if (offsets == nullptr && num_experts != 1) return (int32_t)hipErrorInvalidValue;
     const RowsArgs a = {static_cast<const char*>(x_codes), static_cast<const char*>(w_codes),
                         static_cast<const char*>(x_scales), static_cast<const char*>(w_scales), offsets,
-                        static_cast<char*>(y), rows, blocks * 16, (int)num_experts, (int)n, 0, 0};
+                        static_cast<char*>(y), rows, blocks * 16, (int)num_experts, (int)n, 0, 0, 0};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool whole = blocks % 4 == 0 && host_aligned(x_codes, 16) && host_aligned(w_codes, 16) &&
                        host_aligned(x_scales, 4) && host_aligned(w_scales, 4);

@@ -1055,6 +1055,7 @@ struct RowsArgs {
   char* out;
   int64_t rows, length;  // elements of T
   int groups, cols, tiles_q, most;
+  int first;  // the tile of the launch's first workgroup
 };
 
 // Waves on a SIMD that a tile of so many fragments a wave leaves registers for: two
@@ -1077,15 +1078,16 @@ __global__ __launch_bounds__(WP* WQ * 64, tile_waves(FP* FQ, DIRECT)) void rows_
   constexpr int kHeight = ONCE ? 2 : 8;
   RowTileAt at;
   int tp, tq;
+  const int id = a.first + (int)blockIdx.x;
   if (a.offsets != nullptr) {
     const RowTiles<BP, NW * 64> tiles(shared, a.offsets, a.groups, a.rows, a.most);
     const int total = tiles.total * a.tiles_q;
-    if ((int)blockIdx.x >= total) return;
-    tile_order<kHeight>(xcd_contiguous(blockIdx.x, total), tiles.total, a.tiles_q, &tp, &tq);
+    if (id >= total) return;
+    tile_order<kHeight>(xcd_contiguous(id, total), tiles.total, a.tiles_q, &tp, &tq);
     at = tiles.at(tp);
     if (at.count == 0) return;
   } else {
-    tile_order<kHeight>(xcd_contiguous(blockIdx.x, gridDim.x), a.most, a.tiles_q, &tp, &tq);
+    tile_order<kHeight>(xcd_contiguous(id, a.most * a.tiles_q), a.most, a.tiles_q, &tp, &tq);
     at.row = (int64_t)tp * BP;
     at.count = a.rows - at.row < BP ? (int)(a.rows - at.row) : BP;
     at.group = 0;
@@ -1320,15 +1322,16 @@ __global__ __launch_bounds__(NW * 64, DEPTH ? 1 : 2) void rows_stream(RowsArgs a
 
   RowTileAt at;
   int tp, tq;
+  const int id = a.first + (int)blockIdx.x;
   if (a.offsets != nullptr) {
     const RowTiles<BP, NW * 64> tiles(shared, a.offsets, a.groups, a.rows, a.most);
     const int total = tiles.total * a.tiles_q;
-    if ((int)blockIdx.x >= total) return;
-    tile_order(xcd_contiguous(blockIdx.x, total), tiles.total, a.tiles_q, &tp, &tq);
+    if (id >= total) return;
+    tile_order(xcd_contiguous(id, total), tiles.total, a.tiles_q, &tp, &tq);
     at = tiles.at(tp);
     if (at.count == 0) return;
   } else {
-    tile_order(xcd_contiguous(blockIdx.x, gridDim.x), a.most, a.tiles_q, &tp, &tq);
+    tile_order(xcd_contiguous(id, a.most * a.tiles_q), a.most, a.tiles_q, &tp, &tq);
     at.row = (int64_t)tp * BP;
     at.count = a.rows - at.row < BP ? (int)(a.rows - at.row) : BP;
     at.group = 0;
@@ -1423,10 +1426,23 @@ __global__ __launch_bounds__(256) void narrow_weights(NarrowArgs a) {
   }
 }
 
-constexpr int64_t kMaxThreads = int64_t(1) << 32;  // of one launch
-
 inline unsigned narrow_grid(int64_t elements) {
   return (unsigned)(elements < 4 * 65536 ? (elements + 3) / 4 : 65536);
+}
+
+// launch(first, count) for all of `tiles` workgroups of `threads`: a launch has fewer than
+// 2^32 threads, and takes a multiple of 8 tiles so that each keeps its XCD. No operands that
+// a card holds make 2^31 tiles.
+template <class Launch>
+int32_t launch_tiles(int64_t tiles, int threads, Launch&& launch) {
+  if (tiles > INT32_MAX) return (int32_t)hipErrorInvalidValue;
+  const int64_t most = (int64_t(1) << 32) / threads - 8;
+  for (int64_t first = 0; first < tiles; first += most) {
+    launch((int)first, (unsigned)(tiles - first < most ? tiles - first : most));
+    const int32_t status = launch_status();
+    if (status != (int32_t)hipSuccess) return status;
+  }
+  return (int32_t)hipSuccess;
 }
 
 // The grid of `kernel`, whose workgroups of `threads` own BP rows and BQ columns.
@@ -1436,11 +1452,12 @@ int32_t launch_rows_grid(void (*kernel)(RowsArgs), int threads, RowsArgs a, hipS
   int64_t most = (a.rows + edges * (BP - 1)) / BP;
   most = most < a.rows ? most : a.rows;
   const int64_t tiles_q = ((int64_t)a.cols + BQ - 1) / BQ;
-  if (most * tiles_q * threads >= kMaxThreads) return (int32_t)hipErrorInvalidValue;
   a.most = (int)most;
   a.tiles_q = (int)tiles_q;
-  kernel<<<(unsigned)(most * tiles_q), threads, 0, st>>>(a);
-  return launch_status();
+  return launch_tiles(most * tiles_q, threads, [&](int first, unsigned count) {
+    a.first = first;
+    kernel<<<count, threads, 0, st>>>(a);
+  });
 }
 
 template <class T, class C, bool QROWS, int WP, int WQ, int FP, int FQ, bool DIRECT, bool ONCE = false>

@@ -224,6 +224,52 @@ def test_weights_past_2_31_elements():
         assert torch.equal(gw[e], (part.T @ part).bfloat16()), e
 
 
+def test_more_tiles_than_a_launch_has_room_for():
+    """Sizes of 2^32 threads and more (2^24 tiles of 256), which take several launches: rows, an expert's columns in
+    the product of few rows, and weights. Small integers, whose sums are exact."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    ints = lambda *shape: torch.randint(-4, 5, shape, generator=g, device="cuda", dtype=torch.int8)
+    # 2^30 + 70 rows of 4 float32: 2^24 + 2 tiles of 64 x 64
+    rows = (1 << 30) + 70
+    x = torch.empty(rows, 4, device="cuda")
+    for part in x.split(1 << 27):
+        part.copy_(ints(*part.shape))
+    w = ints(3, 4, 4).float()
+    cuts = [3, 1 << 29, 1 << 29, rows - 5]
+    o = torch.tensor(cuts, device="cuda")
+    for fn, weight in ((K.grouped_linear, w.transpose(1, 2)), (K.grouped_linear_grad_input, w)):  # [e][contracted][out]
+        y = fn(x, w, o)
+        assert (y[:3] == 0).all() and (y[rows - 5:] == 0).all()
+        for e in (0, 2):
+            for first in range(cuts[e], cuts[e + 1], 1 << 27):
+                part = slice(first, min(first + (1 << 27), cuts[e + 1]))
+                want = sum(x[part, c, None] * weight[e, c] for c in range(4))
+                assert torch.equal(y[part], want), (e, first)
+        del y, want
+    del x
+    torch.cuda.empty_cache()
+    # 1024 experts of 4 x 2^20 weights: 2^24 tiles
+    experts, wide = 1024, 1 << 20
+    x, gy = ints(20, wide).float(), ints(20, 4).float()
+    o = torch.zeros(experts + 1, dtype=torch.int64)
+    o[1:], o[600:], o[1024:] = 7, 13, 20  # experts 0, 599 and 1023 have rows
+    o = o.cuda()
+    gw = K.grouped_linear_grad_weight(gy, x, o)
+    for e, part in ((0, slice(0, 7)), (599, slice(7, 13)), (1023, slice(13, 20))):
+        assert torch.equal(gw[e], sum(gy[s, :, None] * x[s] for s in range(part.start, part.stop))), e
+        gw[e] = 0
+    assert not any(bool(part.any()) for part in gw.split(128))
+    del x, gw
+    torch.cuda.empty_cache()
+    # 700 experts of 2^21 x 8 half weights: 700 x 65536 tiles of 16 x 32
+    experts, n = 700, 1 << 21
+    w = ints(experts, n, 8).half()
+    x = ints(experts, 8).half()
+    y = K.grouped_linear(x, w, torch.arange(experts + 1, device="cuda"))
+    for e in (0, 1, 255, 256, 511, 512, 698, 699):
+        assert torch.equal(y[e], (x[e].float() * w[e].float()).sum(-1).half()), e
+
+
 def test_mxfp4_past_2_31_elements():
     rows, k = 540_000, 4096
     g = torch.Generator(device="cuda").manual_seed(0)

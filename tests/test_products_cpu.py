@@ -59,6 +59,37 @@ def test_mxfp4_launchers_refuse_before_device_calls():
     assert lin(None, None, None, None, 8, None, 4, 1025, 16, 4, 2, None) == 1
 
 
+NO_DEVICE = 100  # hipErrorNoDevice: the launcher took the sizes and went on to the launch
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="without operands the launch must not happen")
+@pytest.mark.parametrize("name,rows,experts,n,k,dtype", [
+    ("fwd", 1 << 30, 2, 4, 4, 0), ("fwd", (1 << 31) - 1, 2, 4, 4, 0), ("fwd", (1 << 31) - 1, 2, 8, 8, 2),
+    ("fwd", 8192, 1024, 1 << 21, 8, 1), ("grad_input", 1 << 30, 2, 4, 4, 0), ("grad_input", (1 << 31) - 1, 2, 8, 8, 1),
+    ("grad_weight", 1, 1024, 4, 1 << 20, 0), ("grad_weight", 1, 1024, 1 << 20, 4, 0),
+    ("grad_weight", 1 << 20, 1024, 8192, 8192, 2)])
+def test_more_tiles_than_a_launch_has_room_for(name, rows, experts, n, k, dtype):
+    """Sizes of 2^32 threads and more, whose operands a card holds."""
+    fn = getattr(_cck.load(), f"launch_grouped_linear_{name}")
+    assert fn(None, None, None, None, rows, experts, n, k, dtype, None) == NO_DEVICE
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="without operands the launch must not happen")
+@pytest.mark.parametrize("rows,experts,n,blocks", [((1 << 31) - 1, 1, 16, 4), ((1 << 31) - 1, 1, 8, 1),
+                                                   (8192, 1024, 1 << 21, 1)])
+def test_more_mxfp4_tiles_than_a_launch_has_room_for(rows, experts, n, blocks):
+    lin = _cck.load().launch_mxfp4_linear_fwd
+    offsets = 8 if experts > 1 else None
+    assert lin(None, None, None, None, offsets, None, rows, experts, n, blocks, 2, None) == NO_DEVICE
+
+
+def test_more_tiles_than_any_card_holds():
+    lib = _cck.load()
+    assert lib.launch_grouped_linear_fwd(None, None, None, None, (1 << 31) - 1, 2, 1 << 20, 8, 0, None) == 1
+    assert lib.launch_grouped_linear_grad_input(None, None, None, None, (1 << 31) - 1, 2, 8, 1 << 20, 0, None) == 1
+    assert lib.launch_grouped_linear_grad_weight(None, None, None, None, 1, 1024, 1 << 20, 1 << 20, 0, None) == 1
+
+
 def _raises(fn, *args, match):
     with pytest.raises(ValueError, match=match):
         fn(*args)
