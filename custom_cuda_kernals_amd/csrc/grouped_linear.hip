@@ -95,8 +95,9 @@ int32_t grouped_rows(const void* x, const void* w, const int64_t* offsets, void*
   return with_elem(dtype, [&](auto elem, auto codec) {
     using T = decltype(elem);
     using C = decltype(codec);
-    if (rows <= 0 || length <= 0 || cols <= 0) return (int32_t)hipSuccess;
+    if (rows <= 0 || length < 0 || cols <= 0) return (int32_t)hipSuccess;
     if (!sizes_ok(rows, groups, cols * T::kBytes, length * T::kBytes)) return (int32_t)hipErrorInvalidValue;
+    if (length == 0) return launch_zero_rows<C>(out, rows * cols, static_cast<hipStream_t>(stream));
     const RowsArgs a = {static_cast<const char*>(x), static_cast<const char*>(w), nullptr, nullptr, offsets,
                         static_cast<char*>(out), rows, length, (int)groups, (int)cols, 0, 0, 0};
     const hipStream_t st = static_cast<hipStream_t>(stream);

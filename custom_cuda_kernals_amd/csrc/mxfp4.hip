@@ -207,9 +207,10 @@ extern "C" int32_t launch_mxfp4_linear_fwd(const void* x_codes, const void* x_sc
                                            void* stream) {
   return with_codec(dtype, [&](auto codec) {
     using C = decltype(codec);
-    if (rows <= 0 || n <= 0 || blocks <= 0) return (int32_t)hipSuccess;
+    if (rows <= 0 || n <= 0 || blocks < 0) return (int32_t)hipSuccess;
     if (!sizes_ok(rows, num_experts, n * C::kBytes, blocks * 16)) return (int32_t)hipErrorInvalidValue;
     if (offsets == nullptr && num_experts != 1) return (int32_t)hipErrorInvalidValue;
+    if (blocks == 0) return launch_zero_rows<C>(y, rows * n, static_cast<hipStream_t>(stream));
     const RowsArgs a = {static_cast<const char*>(x_codes), static_cast<const char*>(w_codes),
                         static_cast<const char*>(x_scales), static_cast<const char*>(w_scales), offsets,
                         static_cast<char*>(y), rows, blocks * 16, (int)num_experts, (int)n, 0, 0, 0};

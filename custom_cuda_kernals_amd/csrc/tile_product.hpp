@@ -1426,6 +1426,20 @@ __global__ __launch_bounds__(256) void narrow_weights(NarrowArgs a) {
   }
 }
 
+// Rows of sums of nothing.
+template <class C>
+__global__ __launch_bounds__(256) void zero_rows(char* __restrict__ out, int64_t elements) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < elements; i += (int64_t)gridDim.x * 256) {
+    C::store1(out, i, 0.0f);
+  }
+}
+template <class C>
+int32_t launch_zero_rows(void* out, int64_t elements, hipStream_t st) {
+  if (out == nullptr) return (int32_t)hipSuccess;
+  zero_rows<C><<<flat_grid(elements, 256, 65536), 256, 0, st>>>(static_cast<char*>(out), elements);
+  return launch_status();
+}
+
 inline unsigned narrow_grid(int64_t elements) {
   return (unsigned)(elements < 4 * 65536 ? (elements + 3) / 4 : 65536);
 }

@@ -31,7 +31,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor)
     _check_dims(x, weight, 2, 3)
     y = torch.empty((x.shape[0], weight.shape[1]), dtype=x.dtype, device=x.device)
     native.grouped_linear_fwd(x, weight, offsets, y)
-    return y if x.shape[1] else y.zero_()  # nothing to sum: no launch
+    return y
 
 
 def grouped_linear_grad_input(grad_y: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
@@ -46,7 +46,7 @@ def grouped_linear_grad_input(grad_y: torch.Tensor, weight: torch.Tensor, offset
     _check_dims(grad_y, weight, 2, 3)
     grad_x = torch.empty((grad_y.shape[0], weight.shape[2]), dtype=grad_y.dtype, device=grad_y.device)
     native.grouped_linear_grad_input(grad_y, weight, offsets, grad_x)
-    return grad_x if grad_y.shape[1] else grad_x.zero_()
+    return grad_x
 
 
 def grouped_linear_grad_weight(grad_y: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:

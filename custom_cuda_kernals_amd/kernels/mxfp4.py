@@ -78,4 +78,4 @@ def mxfp4_linear(x_codes: torch.Tensor, x_scales: torch.Tensor, w_codes: torch.T
                          f"{tuple(x_codes.shape)} and {tuple(w_codes.shape)}")
     y = torch.empty((x_codes.shape[0], w_codes.shape[-2]), dtype=out_dtype, device=x_codes.device)
     native.mxfp4_linear_fwd(x_codes, x_scales, w_codes, w_scales, offsets, y)
-    return y if x_codes.shape[1] else y.zero_()  # nothing to sum: no launch
+    return y

@@ -215,8 +215,9 @@ int32_t launch_moe_permutation_offsets_fwd(const int64_t* topk_indices, int64_t*
  * offsets[num_experts] on belong to none. Whatever the offsets hold, nothing
  * outside the `rows` rows is read or written; where they decrease, the results are
  * unspecified. weight: [num_experts, n, k]. rows <= INT32_MAX, num_experts <= 1024
- * and n, k of at most 4 MiB a row, else hipErrorInvalidValue. Outputs must not
- * overlap inputs. ---- */
+ * and n, k of at most 4 MiB a row, else hipErrorInvalidValue. A sum of nothing (n
+ * or k of 0 where it is summed over, no rows) is zero. Outputs must not overlap
+ * inputs. ---- */
 
 /* y[s] = x[s] * weight[e]^T for each row s of expert e; zeros for rows of none.
  * x: [rows, k], y: [rows, n]. */
@@ -255,7 +256,7 @@ int32_t launch_mxfp4_dequant_fwd(const void* codes, const void* scales, void* ou
 /* y[s] = x[s] * w[e]^T of the values that codes and scales stand for, sums in
  * float32, y [rows, n] of dtype. x: codes [rows, 16 * blocks], scales [rows, blocks];
  * w: codes [num_experts, n, 16 * blocks], scales [num_experts, n, blocks]. offsets as
- * above, or NULL with num_experts == 1 for a dense product. */
+ * above, or NULL with num_experts == 1 for a dense product. Without blocks y is zeros. */
 int32_t launch_mxfp4_linear_fwd(const void* x_codes, const void* x_scales, const void* w_codes, const void* w_scales,
                                 const int64_t* offsets, void* y, int64_t rows, int64_t num_experts, int64_t n,
                                 int64_t blocks, int32_t dtype, void* stream);

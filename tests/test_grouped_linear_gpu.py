@@ -175,6 +175,21 @@ def test_nothing_to_sum():
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_launchers_write_sums_of_nothing(dtype):
+    """Through the C launchers, at any element; nothing around the output."""
+    from tests import _cck
+
+    lib, tag = _cck.load(), DTYPES.index(dtype)
+    rows, cols, st = 300, 70, torch.cuda.current_stream().cuda_stream
+    o = torch.tensor([0, 120, 290], device="cuda")
+    for n, k, fn in ((cols, 0, lib.launch_grouped_linear_fwd), (0, cols, lib.launch_grouped_linear_grad_input)):
+        out = torch.full((rows * cols + 16,), 55, dtype=dtype, device="cuda")
+        assert fn(None, None, o.data_ptr(), out.data_ptr() + out.element_size(), rows, 2, n, k, tag, st) == 0
+        torch.cuda.synchronize()
+        assert (out[1:1 + rows * cols] == 0).all() and out[0] == 55 and (out[1 + rows * cols:] == 55).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_infinities_and_nan_stay_in_their_rows(dtype):
     """A NaN or infinity in one row, one expert or one column reaches what it is multiplied with, and nothing else;
     rows of no expert are zeros whatever they hold."""

@@ -214,6 +214,20 @@ def test_nothing_to_sum():
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_launcher_writes_sums_of_nothing(dtype):
+    from tests import _cck
+
+    rows, n, st = 300, 70, torch.cuda.current_stream().cuda_stream
+    o = torch.tensor([0, 120, 290], device="cuda")
+    for offsets, experts in ((None, 1), (o.data_ptr(), 2)):
+        out = torch.full((rows * n + 16,), 55, dtype=dtype, device="cuda")
+        assert _cck.load().launch_mxfp4_linear_fwd(None, None, None, None, offsets, out.data_ptr(), rows, experts, n, 0,
+                                                   DTYPES.index(dtype), st) == 0
+        torch.cuda.synchronize()
+        assert (out[:rows * n] == 0).all() and (out[rows * n:] == 55).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("k", [128, 256, 384, 640])
 def test_large_tiles(k, dtype):
     """Rows and columns enough for the largest tiles, full and cut; odd and even numbers of steps."""

@@ -83,6 +83,15 @@ def test_more_mxfp4_tiles_than_a_launch_has_room_for(rows, experts, n, blocks):
     assert lin(None, None, None, None, offsets, None, rows, experts, n, blocks, 2, None) == NO_DEVICE
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the output is no memory of a device")
+def test_sums_of_nothing_are_written():
+    """A product over no elements has an output all the same: the launcher goes on to the launch."""
+    lib = _cck.load()
+    assert lib.launch_grouped_linear_fwd(None, None, 8, 64, 4, 8, 16, 0, 2, None) == NO_DEVICE
+    assert lib.launch_grouped_linear_grad_input(None, None, 8, 64, 4, 8, 0, 16, 2, None) == NO_DEVICE
+    assert lib.launch_mxfp4_linear_fwd(None, None, None, None, None, 64, 4, 1, 16, 0, 2, None) == NO_DEVICE
+
+
 def test_more_tiles_than_any_card_holds():
     lib = _cck.load()
     assert lib.launch_grouped_linear_fwd(None, None, None, None, (1 << 31) - 1, 2, 1 << 20, 8, 0, None) == 1
