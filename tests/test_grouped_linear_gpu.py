@@ -320,3 +320,60 @@ def test_large_tiles_twice_alike():
 def test_few_tiles_and_many(sizes, n, k, dtype):
     """Either side of where smaller tiles are taken."""
     _check_ints(sizes, n, k, dtype, seed=n)
+
+
+# 16-bit tiles of 128 x 128: 192 of them and more, groups too small for the largest. On average at most 96 rows a group
+# (whole rows: weights read past the caches) and more; cut rows of tiles, groups of none and of one row.
+MIDDLE = {"small groups": [130, 0, 250, 1, 20], "large groups": [300, 130, 0, 77, 100]}
+# Contracted lengths: one step of 128 bytes and of 64 and parts of them, odd and even numbers of steps.
+WHOLE, ODD = [8, 64, 136, 200], [9, 31, 33, 133, 161]
+
+
+def _check_middle(op, sizes, cols, length, dtype, off=0):
+    """One operator of `cols` output columns against float64, from buffers that begin `off` elements past a vector."""
+    offsets = _offsets(sizes, 2)
+    rows = int(offsets[-1]) + 40
+    a = _ints((rows, length), 4, dtype, cols + length)
+    w = _ints((len(sizes), *((cols, length) if op == "linear" else (length, cols))), 4, dtype, cols)
+
+    def moved(t):
+        b = torch.empty(t.numel() + off, dtype=dtype, device="cuda")
+        b[off:] = t.reshape(-1).cuda()
+        return b[off:].view(t.shape)
+
+    name = {"linear": "grouped_linear", "grad_input": "grouped_linear_grad_input"}[op]
+    got = getattr(K, name)(moved(a), moved(w), offsets.cuda()).cpu()
+    want = _rounded(getattr(products, name)(_np(a), _np(w), offsets.numpy()), dtype)
+    assert torch.equal(got, want), (got != want).nonzero()[:4].tolist()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("length", WHOLE)
+@pytest.mark.parametrize("groups", MIDDLE)
+@pytest.mark.parametrize("op", ["linear", "grad_input"])
+def test_middle_tiles(op, groups, length, dtype):
+    _check_middle(op, MIDDLE[groups], 8200, length, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("length,cols", [*((n, 8203) for n in ODD), (64, 8203), (133, 8197), (133, 8200), (133, 8321)])
+@pytest.mark.parametrize("groups", MIDDLE)
+@pytest.mark.parametrize("op", ["linear", "grad_input"])
+def test_middle_tiles_of_odd_widths(op, groups, length, cols, dtype):
+    """The last column tile has 11, 5, 8 and 1 columns: less than a vector and more."""
+    _check_middle(op, MIDDLE[groups], cols, length, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("off", [1, 2, 5])
+@pytest.mark.parametrize("op", ["linear", "grad_input"])
+def test_middle_tiles_of_unaligned_buffers(op, off, dtype):
+    _check_middle(op, MIDDLE["large groups"], 8200, 136, dtype, off=off)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("sizes,n,k", [([200, 0, 333], 1003, 1029), ([40, 0, 65, 1], 1029, 1001), ([130, 7], 1000, 1032),
+                                       ([64, 63, 0, 65], 1032, 1048)], ids=lambda v: str(v)[:16])
+def test_middle_tiles_grad_weight(sizes, n, k, dtype):
+    """96 tiles of 128 x 128 and more: whole vectors and odd widths, steps cut at every part."""
+    _check_ints(sizes, n, k, dtype, seed=k)

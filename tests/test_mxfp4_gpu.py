@@ -245,3 +245,11 @@ def test_rows_a_group(per):
     for k in (256, 224):
         _check_linear([per], 150, k, torch.bfloat16, seed=per, dense=True, low=126, high=128)
         _check_linear([0, 2 * per, per, per + 1, per - 1], 150, k, torch.bfloat16, seed=per, low=126, high=128)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n,k", [(8200, 90), (8200, 160), (8200, 288), (8203, 32), (8193, 256), (8200, 256), (8200, 384)])
+@pytest.mark.parametrize("sizes", [[130, 0, 250, 1, 20], [300, 130, 0, 77, 100]], ids=["small", "large"])
+def test_middle_tiles(sizes, n, k, dtype):
+    """192 tiles of 128 x 128 and more: whole steps of four blocks, and any number of blocks."""
+    _check_linear(sizes, n, k, dtype, seed=k, first=2, rows=sum(sizes) + 42, low=126, high=128)
