@@ -253,3 +253,29 @@ def test_rows_a_group(per):
 def test_middle_tiles(sizes, n, k, dtype):
     """192 tiles of 128 x 128 and more: whole steps of four blocks, and any number of blocks."""
     _check_linear(sizes, n, k, dtype, seed=k, first=2, rows=sum(sizes) + 42, low=126, high=128)
+
+
+SCALE_BYTES = [0, 1, 2, 126, 128, 252, 253, 254]
+
+
+@pytest.mark.parametrize("rows,n", [(8, 8), (16, 8200), (24, 40), (40, 40), (40, 24576), (256, 38400)],
+                         ids=["stream16x16", "stream16x32", "stream32x32", "tiles64", "tiles128", "tiles256"])
+@pytest.mark.parametrize("k", [32, 96, 128, 384])
+def test_scales_of_every_size(rows, n, k):
+    """The ends of E8M0, and scales whose product is ordinary where neither is: a row's blocks share a scale, and all
+    codes are positive, so a sum grows to its value, which float32 holds, or which is past its range: infinity. A sum
+    below the smallest normal number may be off by that (the bound's last term)."""
+    g = _gen(rows + k)
+    pairs = []
+    for count in (rows, n):
+        codes = torch.randint(0, 8, (count, -(-k // 32) * 32), generator=g, dtype=torch.uint8)
+        scales = torch.tensor(SCALE_BYTES, dtype=torch.uint8)[torch.arange(count) % 8, None].expand(-1, -(-k // 32))
+        pairs.append((codes[:, 0::2] | codes[:, 1::2] << 4, scales.contiguous().view(torch.float8_e8m0fnu)))
+    got = K.mxfp4_linear(*(t.cuda() for p in pairs for t in p), out_dtype=torch.float32).cpu().double().numpy()
+    exact = _values(pairs[0], k) @ _values(pairs[1], k).T
+    past = exact >= 2.0 ** 128
+    assert (got[past] == np.inf).all() and past.any()
+    got, exact = got[~past], exact[~past]
+    bound = (k + 2) * U * exact + torch.finfo(torch.float32).tiny
+    off = ~(np.abs(got - exact) <= bound)
+    assert not off.any(), (int(off.sum()), got[off][:4], exact[off][:4])
