@@ -43,7 +43,8 @@ constexpr int64_t kMaxRowLength = int64_t(1) << 22;
 // accumulators a lane do not stay there: it moves them to the other registers and back
 // around every product. The compiler does not see that these are matrix instructions, so
 // the wait states that they need are written out: two behind a vector instruction that
-// writes an operand (operands_ready), 18 before the sums are read (acc_ready).
+// writes an operand (operands_ready), 18 before the sums are read (acc_ready). That no copy
+// of the compiler's is nearer is tested on the built code (tests/test_matrix_asm_cpu.py).
 __device__ inline void operands_ready() { asm volatile("s_nop 1"); }
 template <int N>
 __device__ inline void computed_here(int (&v)[N]) {  // and not behind the wait
@@ -261,8 +262,8 @@ constexpr uint32_t kOutOfRange = 0x80000000u;  // an offset past the end of ever
 // which does not know that the slots of a ring are apart, would wait for these loads
 // before every later LDS read; their one wait is loads_landed (all but the last LEFT
 // of the wave's loads).
-// In two instructions, the first naming the place (register M0, which the compiler does
-// not use): one other instruction at least belongs between them.
+// In two instructions, the first naming the place (register M0, which the compiler reserves
+// and does not use by itself): one other instruction at least belongs between them.
 __device__ inline void lds_place(LdsPtr to) {
   asm volatile("s_mov_b32 m0, %0" ::"s"(__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)to)) : "memory");
 }
@@ -876,12 +877,20 @@ struct Product {
     first.read(at0, 0);
     const int whole = looped(steps);
     int t = 0;
-    for (; t < whole; t += 2) {
+    auto two = [&] {
       step(at0, at1);
       step(at1, at0);
-      folded.every(2 * t + 4, acc);
-    }
-    if constexpr (!kWide) {
+      t += 2;
+      folded.every(2 * t, acc);
+    };
+    if constexpr (kWide) {
+      // At least once, as steps > 0: with a way around the loop the compiler copies the sums where
+      // both ways meet, in front of the wait that acc_ready is.
+      do {
+        two();
+      } while (t < whole);
+    } else {
+      while (t < whole) two();
       if (t < steps) {
         second.read(at0, 1);
         first.multiply(acc, [](int) {});
