@@ -11,9 +11,12 @@
 // and an expert without rows has a zero gradient. The group sizes stay on the
 // GPU: the grid has room for the most tiles that `rows` rows can make.
 //
-// 8192 rows on 8 experts of 14336 x 4096, bf16: 786, 858 and 854 us (1.22, 1.12 and 1.13
-// PFLOP/s), bound by the matrix cores at the clock the power limit leaves them, and by the
-// groups' cut tiles; 16 rows: 118 us, bound by the weights' 7.1 TB/s.
+// 8192 unevenly routed rows on 8 experts of 14336 x 4096, bf16: 790, 871 and 861 us (1.22,
+// 1.10 and 1.12 PFLOP/s), with the matrix cores busy 72, 58 and 60 % of the cycles, at the
+// clock that the power limit leaves (1.7 GHz). The loop itself keeps them busy 92, 90 and
+// 87 % (see Product). What else there is: a tile's ends, as long as 7 to 9 of its steps (64
+// steps in y, 16 on average in grad_w); cut tiles; and in grad_x 2.25 rounds of tiles that
+// take three. 16 rows: 113 us, bound by reading the weights.
 #include "tile_product.hpp"
 
 namespace cck {
@@ -136,9 +139,14 @@ int32_t run_weights(const void* grad, const void* x, const int64_t* offsets, voi
 // Tiles of 256 x 256 where experts have 768 rows or more on average and each CU gets a tile
 // (bf16, us, against 128 x 128: 8 experts of 1024 rows, 2048 x 1408 65.7 and 67.8, of 512 rows,
 // 2048 x 2048 49.3 and 46.5; one of 4096 rows, 4096 x 4096 98.9 and 131); of 64 x 64 where
-// fewer than 96 of 128 x 128 would share the 256 CUs (8192 rows, 1024 x 1024, 64 tiles: 54.5
-// and 67.0; 4 experts of 500 rows, 1024 x 1536, 384 tiles: 15.8 and 13.7), and always for
-// fp32 (8192 rows, 1024 x 1024: 174 and 513; 4096 x 4096: 982 and 963).
+// fewer than 96 of 128 x 128 would share the 256 CUs. bf16, us, 64 x 64 and 128 x 128: 64 tiles
+// of 128 x 128, 8192 rows 54.5 and 67.6, of 500 rows 4.9 and 7.4; 96 tiles, one expert of 8192
+// rows 55.7 and 67.5, 6 of 1365 rows 15.2 and 14.0, of 500 rows 5.8 and 7.5; 128 tiles, one of
+// 8192 rows 57.1 and 69.1, 8 of 1024 rows 14.4 and 11.2, of 500 rows 8.3 and 7.6; 160 tiles,
+// one of 8192 rows 93.4 and 68.7, 10 of 819 rows 16.2 and 9.6, of 500 rows 11.5 and 7.6. So
+// from 96 to 128 tiles it is the number of experts that decides, which the rule leaves out.
+// Always 64 x 64 for fp32 (us, against 128 x 128: 8192 rows, 1024 x 1024 170 and 514; 8 experts
+// of 512 rows, 2048 x 1408 186 and 197; one of 4096 rows, 4096 x 4096 989 and 960).
 template <class T, class C, bool WHOLE>
 int32_t run_weights_by_size(const void* grad, const void* x, const int64_t* offsets, void* out, int64_t rows,
                             int64_t groups, int64_t n, int64_t k, hipStream_t st) {

@@ -12,8 +12,8 @@
 //
 // Quantiser and inverse are bound by HBM: [14336, 4096] bf16 and back take 49 us (6.1 TB/s). The
 // product (tile_product.hpp) takes codes and scales as they are to the scaled matrix
-// instructions: 16 rows, 14336 x 4096 8.5 us, where the launch's ramp is half; 8192 rows on
-// 8 experts 312 us, 3.1 PFLOP/s, of tiles whose ends cost as much as ten of their 16 steps.
+// instructions: 16 rows, 14336 x 4096 8.6 us, where the launch's ramp is half; 8192 rows on
+// 8 experts 316 us, 3.0 PFLOP/s, of tiles whose ends cost as much as ten of their 16 steps.
 #include "tile_product.hpp"
 
 namespace cck {

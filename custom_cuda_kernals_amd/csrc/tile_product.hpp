@@ -705,9 +705,10 @@ struct Product {
 
   // Half a step's products are issued in kParts parts, with reads and loads between them:
   // one by one where a SIMD has a single wave to issue anything (kWide), else by rows.
-  // 256 x 256 tiles take 2250 cycles a step so, of which the matrix cores need 2048 (8192 rows
-  // on 8 groups of 14336 x 4096, bf16: 786 us, 1.22 PFLOP/s; 128 x 128 tiles, two workgroups a
-  // CU, which LDS bounds, 1057).
+  // 256 x 256 tiles of rows take 2215 cycles a step so, of which the matrix cores need 2048; with
+  // Q in columns 2280, with both 2360; and 27000 beside the steps, the launch among them (slopes
+  // of 56 to 224 steps, one tile a CU). 8192 rows on 8 groups of 14336 x 4096, bf16: 790 us,
+  // 1.22 PFLOP/s; 128 x 128 tiles, two workgroups a CU, which LDS bounds, 1057.
   static constexpr bool kWide = FP == 8 && FQ == 8;
   // Sums in the accumulation registers: for the wide ones, and for the scaled products, whose
   // builtin takes operands of twice the size, zeros behind what there is of them.
@@ -1131,9 +1132,9 @@ __global__ __launch_bounds__(WP* WQ * 64, tile_waves(FP* FQ, DIRECT)) void rows_
 // Few rows a group: the weights are read once, and that is the time. A workgroup
 // owns FP x 16 rows and FQ x 16 columns; its NW waves take the contracted index in
 // turn, and their sums meet in LDS at the end, in the order of the waves. 16 rows on 8
-// groups of 14336 x 4096, bf16: 118 us, 7.1 TB/s; straight from memory to registers, as
-// rows off their alignment take, 160 to 200. A ring of two steps was as good as any deeper
-// one, and 32 columns a workgroup of four waves as good as other shapes.
+// groups of 14336 x 4096, bf16: 113 us (their reads from HBM alone, at 6.9 TB/s, 123); straight
+// from memory to registers, as rows off their alignment take, 160 to 200. A ring of two steps was
+// as good as any deeper one, and 32 columns a workgroup of four waves as good as other shapes.
 // ---------------------------------------------------------------------------
 
 constexpr int kStreamBytes = 256, kStreamSteps = kStreamBytes / 64;
@@ -1495,12 +1496,18 @@ int32_t launch_stream(const RowsArgs& a, hipStream_t st) {
 }
 
 // Tiles of 256 x 256, of which a SIMD's one wave reads a quarter less from LDS for a
-// product, pay where they are filled and enough for the 256 CUs (one cut short a group).
-// bf16, us, forward and input gradient, against 128 x 128: 8 groups of 1024 rows, 14336 x
-// 4096 781 and 882 (128 x 128: 1057 and 1138); of 128 rows 196 and 279 (238 and 296), of 64
-// rows 207 and 242 (187 and 197); 64 groups of 128 rows, 1408 x 2048 116 and 115 (105 and
-// 102), of 256 rows 159 and 121 (166 and 156); 8 of 512 rows, 2048 x 2048, 160 tiles, 49 and
-// 50 (68 and 64), 2048 rows, 4096 x 4096, 128 tiles, 81 and 82 (69 and 73).
+// product, pay where they are filled and enough for the 256 CUs. bf16, us, forward and input
+// gradient, in brackets 128 x 128: 8 groups of 1024 rows, 14336 x 4096 781 and 882 (1057 and
+// 1138), of 128 rows 196 and 279 (238 and 296), of 64 rows 207 and 242 (187 and 197); 64
+// groups of 128 rows, 1408 x 2048 116 and 95 (110 and 97), of 160 rows 119 and 104 (118 and
+// 110), of 256 rows 125 and 110 (141 and 138); 160 of 128 rows, 1536 x 2048 232 and 230 (221
+// and 233), of 160 rows 252 and 252 (299 and 305).
+// The group sizes are not known here: groups / 2 stands for one cut tile a group, half
+// filled. Of equal groups that a tile holds there are fewer tiles, and where those are
+// fewer than the CUs this rule loses: 16 groups, 2048 x 2048, 128 tiles, 192 rows 40 and 41 (31
+// and 31), 256 rows 42 and 43 (35 and 35); 8 of 192 rows, 4096 x 4096, 128 tiles 83 and 82 (72
+// and 70); and so does half a round too many: 32 of 320 rows, 1408 x 2048, 384 tiles 81 and 85
+// (73 and 74).
 template <class T>
 inline bool wide_tiles(const RowsArgs& a) {
   return T::kAccumulates && a.rows >= 128 * (int64_t)a.groups &&
@@ -1521,8 +1528,9 @@ int32_t launch_rows_small(const RowsArgs& a, hipStream_t st) {
   if constexpr (T::kBytes != 4) {
     if (middle_tiles<T>(a)) {
       // Groups that fill one tile on average: their weights are read once, past the caches and
-      // group after group (160 groups of 77 rows, 1536 x 2048: 212 us against 220 through the
-      // caches, 5 of them for the order; 64 groups of 200 rows, 1408 x 2048: 133 against 131).
+      // group after group (160 groups of 77 rows, 1536 x 2048: 184 us against 203 through the
+      // caches; 64 groups of 128 rows, 1408 x 2048: 102 against 110, of 160 rows 163 against 118).
+      // It loses where one group has most of the rows (12161 of those 12320: 278 against 238).
       if constexpr (WHOLE) {
         if (a.rows <= 96 * (int64_t)a.groups) return launch_rows<T, C, QROWS, 2, 2, 4, 4, true, true>(a, st);
       }
@@ -1538,7 +1546,9 @@ int32_t launch_rows_small(const RowsArgs& a, hipStream_t st) {
 // where tiles are few. bf16, us, streams of 16 rows, of 32, and 128 x 128 tiles: 8 groups of 2
 // rows, 14336 x 4096 121, 123, 149, of 8 rows 150, 153, 163, of 16 rows 208, 171, 152, of 32
 // rows 315, 243, 158; 64 groups of 8 rows, 1408 x 2048 60, 70, 85, of 16 rows 77, 75, 83, of 24
-// rows 97, 84, 84; one of 32 rows, 4096 x 4096 11, 14, 49, 14336 x 4096 33, 26, 51. Two fragments
+// rows 97, 84, 84; one of 32 rows, 4096 x 4096 11, 14, 49, 14336 x 4096 33, 26, 51. One group
+// with most of the rows takes the streams longer, and the tiles hardly less then (449 of 512 rows
+// on 64 groups: 74 and 93; 57 of 64 on 8 of 14336 x 4096: 169 and 164). Two fragments
 // of columns a workgroup, or one where that leaves CUs without (one group of 8 rows,
 // 4096 x 4096 10.7 and 9.8; 64 of 8, 1408 x 2048 60 and 65).
 template <class T, class C, bool WHOLE>

@@ -377,3 +377,10 @@ def test_middle_tiles_of_unaligned_buffers(op, off, dtype):
 def test_middle_tiles_grad_weight(sizes, n, k, dtype):
     """96 tiles of 128 x 128 and more: whole vectors and odd widths, steps cut at every part."""
     _check_ints(sizes, n, k, dtype, seed=k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n,k", [(2056, 136), (2051, 133), (2056, 1032), (2051, 1029), (2057, 600)])
+def test_few_rows_of_many_columns(n, k, dtype):
+    """At most 8 rows a group and columns enough for every CU: whole rows and odd ones, and more steps than waves."""
+    _check_ints([1, 0, 8, 3, 9], n, k, dtype, seed=k, first=1, rows=24)
