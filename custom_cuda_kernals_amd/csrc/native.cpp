@@ -939,6 +939,7 @@ void mxfp4_linear_fwd(py::handle x_codes, py::handle x_scales, py::handle w_code
 
 }  // namespace
 
+#include "native_decode.hpp"
 #include "native_calls.hpp"
 
 PYBIND11_MODULE(_native, m) {
@@ -981,6 +982,17 @@ PYBIND11_MODULE(_native, m) {
   m.def("mxfp4_dequant_fwd", &mxfp4_dequant_fwd, py::arg("codes"), py::arg("scales"), py::arg("out"));
   m.def("mxfp4_linear_fwd", &mxfp4_linear_fwd, py::arg("x_codes"), py::arg("x_scales"), py::arg("w_codes"),
         py::arg("w_scales"), py::arg("offsets"), py::arg("y"));
+  m.def("rope_at_fwd", &rope_at_fwd, py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("frequencies"),
+        py::arg("q_out"), py::arg("k_out"), py::arg("layout"), py::arg("scale"), py::arg("inverse"));
+  m.def("rope_to_cache_fwd", &rope_to_cache_fwd, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("key_cache"),
+        py::arg("value_cache"), py::arg("slots"), py::arg("positions"), py::arg("frequencies"), py::arg("q_out"),
+        py::arg("layout"), py::arg("scale"), py::arg("key_scale"), py::arg("value_scale"));
+  m.def("paged_attention_fwd", &paged_attention_fwd, py::arg("q"), py::arg("key_cache"), py::arg("value_cache"),
+        py::arg("page_table"), py::arg("lengths"), py::arg("out"), py::arg("lse"), py::arg("workspace"),
+        py::arg("scale"), py::arg("window"), py::arg("key_scale"), py::arg("value_scale"));
+  m.def("paged_attention_workspace", &cck_paged_attention_workspace, py::arg("sequences"), py::arg("heads"),
+        py::arg("kv_heads"), py::arg("head_dim"), py::arg("page_size"), py::arg("table_width"),
+        "Bytes of the workspace that paged_attention_fwd takes.");
   // The Python API in one call each (native_calls.hpp).
   if (PyModule_AddFunctions(m.ptr(), calls::kMethods) != 0) throw py::error_already_set();
 }

@@ -43,8 +43,8 @@ inline bool ordinary_state() {
          !c10::impl::tls_local_dispatch_key_set().included_.has_any(kWrappers);
 }
 
-// A plain (exactly torch.Tensor or Parameter), contiguous, non-empty, unnamed GPU tensor, or nullptr.
-inline const at::Tensor* plain(PyObject* o) {
+// A plain (exactly torch.Tensor or Parameter), contiguous (or `strided`), non-empty, unnamed GPU tensor, or nullptr.
+inline const at::Tensor* plain(PyObject* o, bool strided = false) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.defined() || t.device().type() != c10::DeviceType::CUDA || t.layout() != c10::kStrided) return nullptr;
@@ -53,7 +53,7 @@ inline const at::Tensor* plain(PyObject* o) {
                                                c10::DispatchKey::FuncTorchGradWrapper}))) {
     return nullptr;
   }
-  return t.is_contiguous() && t.numel() > 0 && !t.has_names() ? &t : nullptr;
+  return (strided || t.is_contiguous()) && t.numel() > 0 && !t.has_names() ? &t : nullptr;
 }
 
 // A plain input as the checks saw it: what they compare and the outputs are
@@ -62,7 +62,7 @@ inline const at::Tensor* plain(PyObject* o) {
 // without the lock, as set_ and resize_, race with any reader of it.)
 class Input {
  public:
-  explicit Input(PyObject* o) : object_(o), t_(plain(o)) {
+  explicit Input(PyObject* o, bool strided = false) : object_(o), strided_(strided), t_(plain(o, strided)) {
     if (t_ == nullptr) return;
     sizes_ = t_->sizes();
     strides_ = t_->strides();
@@ -72,7 +72,7 @@ class Input {
   explicit operator bool() const { return t_ != nullptr; }
   // The tensor still is what the checks saw.
   bool unchanged() const {
-    return plain(object_) == t_ && t_->sizes() == sizes() && t_->strides() == strides() &&
+    return plain(object_, strided_) == t_ && t_->sizes() == sizes() && t_->strides() == strides() &&
            t_->scalar_type() == type_ && t_->device() == device_;
   }
   const at::Tensor& tensor() const { return *t_; }
@@ -88,6 +88,7 @@ class Input {
 
  private:
   PyObject* object_;
+  bool strided_;
   const at::Tensor* t_;
   c10::DimVector sizes_, strides_;
   c10::ScalarType type_ = c10::ScalarType::Undefined;
@@ -576,6 +577,190 @@ inline PyObject* mxfp4_linear(PyObject*, PyArgs a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// [..., heads, head_dim] as validate_heads takes it: its strides of tokens and heads.
+struct HeadsOf {
+  int64_t tokens = 0, heads = 0, dim = 0, token_stride = 0, head_stride = 0;
+  explicit HeadsOf(const Input& t) {
+    if (!t || t.dim() < 3 || float_tag(t) < 0) return;
+    heads = t.size(-2);
+    dim = t.size(-1);
+    token_stride = heads * dim;
+    head_stride = dim;
+    if (!t.tensor().is_contiguous()) {
+      if (t.dim() != 3 || (t.strides()[2] != 1 && dim > 1)) return;
+      token_stride = t.strides()[0];
+      head_stride = t.strides()[1];
+    }
+    tokens = t.numel() / (heads * dim);
+  }
+  explicit operator bool() const { return tokens > 0; }
+};
+
+// A number, as a double.
+inline bool number_arg(PyObject* o, double* value) {
+  if (!PyFloat_CheckExact(o)) return false;
+  *value = PyFloat_AS_DOUBLE(o);
+  return true;
+}
+inline int layout_arg(PyObject* o) {  // 0 half, 1 interleaved, -1 anything else
+  if (!PyUnicode_CheckExact(o)) return -1;
+  if (PyUnicode_CompareWithASCIIString(o, "half") == 0) return 0;
+  return PyUnicode_CompareWithASCIIString(o, "interleaved") == 0 ? 1 : -1;
+}
+inline bool tokens_like(const Input& t, const Input& q) {  // int64, q's shape without its heads
+  return t.type() == c10::ScalarType::Long && t.device() == q.device() &&
+         t.sizes() == q.sizes().slice(0, q.dim() - 2);
+}
+inline bool frequencies_ok(const Input& f, const Input& q) {
+  return f.type() == c10::ScalarType::Double && f.device() == q.device() && f.dim() == 1 &&
+         2 * f.size(0) <= q.size(-1);
+}
+inline bool like_q(const Input& t, const Input& q) {
+  return t.type() == q.type() && t.device() == q.device() && t.dim() == q.dim() && t.size(-1) == q.size(-1) &&
+         t.sizes().slice(0, t.dim() - 2) == q.sizes().slice(0, q.dim() - 2);
+}
+inline bool rope_sizes_ok(const HeadsOf& q, const HeadsOf& k) {
+  return q.dim <= kMaxRopeDim && q.heads + 2 * k.heads <= (int64_t(1) << 20) / q.dim;
+}
+inline bool apart(const HeadsOf& h) {
+  return ::apart(h.tokens, h.heads, h.dim, h.token_stride, h.head_stride);
+}
+
+// (q, k, positions, frequencies, layout, scale, inverse, inplace); in place: True
+inline PyObject* rope_at(PyObject*, PyArgs a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  double scale = 1.0;
+  if (n != 8 || !number_arg(a[5], &scale) || !PyBool_Check(a[6]) || !PyBool_Check(a[7]) || !ordinary_state()) {
+    Py_RETURN_NONE;
+  }
+  const bool inplace = a[7] == Py_True;
+  const int layout = layout_arg(a[4]);
+  const Input q(a[0], true), k(a[1], true), positions(a[2]), frequencies(a[3]);
+  const HeadsOf qh(q), kh(k);
+  if (layout < 0 || !qh || !kh || !positions || !frequencies || !like_q(k, q) || !tokens_like(positions, q) ||
+      !frequencies_ok(frequencies, q) || !rope_sizes_ok(qh, kh) || (inplace && (!apart(qh) || !apart(kh)))) {
+    Py_RETURN_NONE;
+  }
+  const Launch launch(q.device().index());
+  at::Tensor out[2];
+  int64_t strides[8] = {qh.token_stride, qh.head_stride, kh.token_stride, kh.head_stride,
+                        qh.heads * qh.dim, qh.dim, kh.heads * kh.dim, kh.dim};
+  if (inplace) {
+    std::copy(strides, strides + 4, strides + 4);
+  } else {
+    allocate(q.device(), {{q.sizes(), q.type()}, {k.sizes(), k.type()}}, out);
+  }
+  if (!unchanged(q, k, positions, frequencies)) Py_RETURN_NONE;
+  if (inplace && q.data() == k.data()) Py_RETURN_NONE;
+  check_launch("launch_rope_at_fwd",
+               launch_rope_at_fwd(q.data(), k.data(), inplace ? q.data() : out[0].data_ptr(),
+                                  inplace ? k.data() : out[1].data_ptr(), (const int64_t*)positions.data(),
+                                  frequencies.data(), strides, qh.tokens, qh.heads, kh.heads, qh.dim,
+                                  frequencies.size(0), layout, a[6] == Py_True, (float)scale, float_tag(q), launch.st));
+  if (inplace) Py_RETURN_TRUE;
+  return result(std::move(out[0]), std::move(out[1]));
+  END_HANDLE_TH_ERRORS
+}
+
+// The tag of a cache beside q of `kv_heads` heads, -1 for anything else.
+inline int32_t cache_tag(const Input& c, const Input& q, int64_t kv_heads) {
+  if (!c || c.device() != q.device() || c.dim() != 4 || c.size(2) != kv_heads || c.size(3) != q.size(-1)) return -1;
+  const int32_t tag = tag_of(c.type());
+  return tag == float_tag(q) || is_fp8(tag) ? tag : -1;
+}
+
+// (q, k, v, key_cache, value_cache, slots, positions, frequencies, layout, scale, key_scale, value_scale, inplace);
+// in place: True
+inline PyObject* rope_to_cache(PyObject*, PyArgs a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  double scale = 1.0, key_scale = 1.0, value_scale = 1.0;
+  if (n != 13 || !number_arg(a[9], &scale) || !number_arg(a[10], &key_scale) || !number_arg(a[11], &value_scale) ||
+      !PyBool_Check(a[12]) || !ordinary_state()) {
+    Py_RETURN_NONE;
+  }
+  const bool inplace = a[12] == Py_True;
+  const int layout = layout_arg(a[8]);
+  const Input q(a[0], true), k(a[1], true), v(a[2], true), keys(a[3]), values(a[4]), slots(a[5]), positions(a[6]),
+      frequencies(a[7]);
+  const HeadsOf qh(q), kh(k), vh(v);
+  if (layout < 0 || !qh || !kh || !vh || !slots || !positions || !frequencies || !like_q(k, q) || !like_q(v, q) ||
+      vh.heads != kh.heads || !tokens_like(slots, q) || !tokens_like(positions, q) || !frequencies_ok(frequencies, q) ||
+      !rope_sizes_ok(qh, kh) || (inplace && !apart(qh))) {
+    Py_RETURN_NONE;
+  }
+  const int32_t tag = cache_tag(keys, q, kh.heads);
+  if (tag < 0 || tag != cache_tag(values, q, kh.heads) || keys.sizes() != values.sizes() ||
+      !cache_scale_ok(key_scale, is_fp8(tag)) || !cache_scale_ok(value_scale, is_fp8(tag))) {
+    Py_RETURN_NONE;
+  }
+  const Launch launch(q.device().index());
+  at::Tensor out[1];
+  const int64_t strides[8] = {qh.token_stride, qh.head_stride, kh.token_stride, kh.head_stride,
+                              vh.token_stride, vh.head_stride, inplace ? qh.token_stride : qh.heads * qh.dim,
+                              inplace ? qh.head_stride : qh.dim};
+  if (!inplace) allocate(q.device(), {{q.sizes(), q.type()}}, out);
+  if (!unchanged(q, k, v, keys, values, slots, positions, frequencies)) Py_RETURN_NONE;
+  check_launch("launch_rope_to_cache_fwd",
+               launch_rope_to_cache_fwd(q.data(), k.data(), v.data(), inplace ? q.data() : out[0].data_ptr(),
+                                        keys.data(), values.data(), (const int64_t*)slots.data(),
+                                        (const int64_t*)positions.data(), frequencies.data(), strides, qh.tokens,
+                                        qh.heads, kh.heads, qh.dim, frequencies.size(0), keys.size(0) * keys.size(1),
+                                        layout, (float)scale, (float)key_scale, (float)value_scale, float_tag(q), tag,
+                                        launch.st));
+  if (inplace) Py_RETURN_TRUE;
+  return result(std::move(out[0]));
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, key_cache, value_cache, page_table, lengths, scale, window, key_scale, value_scale, return_lse)
+inline PyObject* paged_attention(PyObject*, PyArgs a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  double scale = 1.0, key_scale = 1.0, value_scale = 1.0;
+  if (n != 10 || !number_arg(a[5], &scale) || !PyLong_CheckExact(a[6]) || !number_arg(a[7], &key_scale) ||
+      !number_arg(a[8], &value_scale) || !PyBool_Check(a[9]) || !ordinary_state()) {
+    Py_RETURN_NONE;
+  }
+  int overflow = 0;
+  const long long window = PyLong_AsLongLongAndOverflow(a[6], &overflow);
+  const bool with_lse = a[9] == Py_True;
+  const Input q(a[0], true), keys(a[1]), values(a[2]), table(a[3]), lengths(a[4]);
+  const HeadsOf qh(q);
+  if (overflow != 0 || window < 0 || !qh || q.dim() != 3 || !keys || keys.dim() != 4 || !values || !table || !lengths) {
+    Py_RETURN_NONE;
+  }
+  const int64_t kv = keys.size(2), page = keys.size(1), width = table.size(-1);
+  const int32_t tag = cache_tag(keys, q, kv);
+  if (tag < 0 || tag != cache_tag(values, q, kv) || keys.sizes() != values.sizes() || !tokens_like(lengths, q) ||
+      table.type() != c10::ScalarType::Long || table.device() != q.device() || table.dim() != 2 ||
+      table.size(0) != qh.tokens || !cache_scale_ok(key_scale, is_fp8(tag)) ||
+      !cache_scale_ok(value_scale, is_fp8(tag)) ||
+      attention_limits(qh.tokens, qh.heads, kv, qh.dim, page, width) != nullptr) {
+    Py_RETURN_NONE;
+  }
+  const int64_t stats[2] = {qh.tokens, qh.heads};
+  const int64_t bytes = cck_paged_attention_workspace(qh.tokens, qh.heads, kv, qh.dim, page, width);
+  const int64_t room[1] = {bytes / 4}, none[1] = {0};
+  const Launch launch(q.device().index());
+  at::Tensor out[3];
+  allocate(q.device(),
+           {{q.sizes(), q.type()},
+            {with_lse ? c10::IntArrayRef(stats) : c10::IntArrayRef(none), c10::ScalarType::Float},
+            {bytes > 0 ? c10::IntArrayRef(room) : c10::IntArrayRef(none), c10::ScalarType::Float}},
+           out);
+  if (!unchanged(q, keys, values, table, lengths)) Py_RETURN_NONE;
+  check_launch("launch_paged_attention_fwd",
+               launch_paged_attention_fwd(q.data(), keys.data(), values.data(), (const int64_t*)table.data(),
+                                          (const int64_t*)lengths.data(), out[0].data_ptr(),
+                                          with_lse ? (float*)out[1].data_ptr() : nullptr,
+                                          bytes > 0 ? out[2].data_ptr() : nullptr, qh.token_stride, qh.head_stride,
+                                          qh.tokens, qh.heads, kv, qh.dim, keys.size(0), page, width, window,
+                                          (float)scale, (float)key_scale, (float)value_scale, float_tag(q), tag,
+                                          launch.st));
+  if (with_lse) return result(std::move(out[0]), std::move(out[1]));
+  return result(std::move(out[0]));
+  END_HANDLE_TH_ERRORS
+}
+
 using FastCall = PyObject* (*)(PyObject*, PyArgs, Py_ssize_t);
 template <FastCall F>
 PyCFunction as_method() {
@@ -600,6 +785,9 @@ inline PyMethodDef kMethods[] = {
     {"mxfp4_quant_call", as_method<mxfp4_quant>(), METH_FASTCALL, nullptr},
     {"mxfp4_dequant_call", as_method<mxfp4_dequant>(), METH_FASTCALL, nullptr},
     {"mxfp4_linear_call", as_method<mxfp4_linear>(), METH_FASTCALL, nullptr},
+    {"rope_at_call", as_method<rope_at>(), METH_FASTCALL, nullptr},
+    {"rope_to_cache_call", as_method<rope_to_cache>(), METH_FASTCALL, nullptr},
+    {"paged_attention_call", as_method<paged_attention>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -261,6 +261,57 @@ int32_t launch_mxfp4_linear_fwd(const void* x_codes, const void* x_scales, const
                                 const int64_t* offsets, void* y, int64_t rows, int64_t num_experts, int64_t n,
                                 int64_t blocks, int32_t dtype, void* stream);
 
+/* ---- Decoding (no reference counterpart): rotary positions, a paged key-value cache
+ * and the attention that reads it. Heads are [tokens, heads, head_dim] with head_dim
+ * contiguous and any stride of tokens and of heads, in elements; `strides` and the
+ * stride arguments are on the host, everything else on the device. ---- */
+
+/* Each pair (a, b) of the first 2 * half elements of a head, (x[i], x[half + i]) or,
+ * interleaved, (x[2i], x[2i + 1]), becomes factor * (a cos - b sin, b cos + a sin) of
+ * the angle positions[token] * frequencies[i]; inverse: of the negative angle, which is
+ * the gradient. The other elements are copied. positions [tokens], frequencies float64
+ * [half] (any position whose angle float64 holds). head_dim <= 2048. strides: token and
+ * head strides of q, k, q_out, k_out (8 values). q_out == q and k_out == k (with their
+ * strides) rotate in place. */
+int32_t launch_rope_at_fwd(const void* q, const void* k, void* q_out, void* k_out, const int64_t* positions,
+                           const void* frequencies, const int64_t* strides, int64_t tokens, int64_t n_q_heads,
+                           int64_t n_kv_heads, int64_t head_dim, int64_t half, int32_t interleaved, int32_t inverse,
+                           float factor, int32_t dtype, void* stream);
+
+/* As above for q; k, rotated, and v go to row slots[token] of the caches [cache_slots,
+ * n_kv_heads, head_dim] (slot = page * page_size + place in the page), of dtype
+ * cache_dtype: dtype, or FP8 codes of the values divided by key_scale / value_scale
+ * (within [1e-30, 1e30]), beyond the format's largest value to it. A token whose slot is
+ * outside [0, cache_slots) is not written. Tokens of one call have slots of their own.
+ * strides: token and head strides of q, k, v, q_out (8 values). */
+int32_t launch_rope_to_cache_fwd(const void* q, const void* k, const void* v, void* q_out, void* key_cache,
+                                 void* value_cache, const int64_t* slots, const int64_t* positions,
+                                 const void* frequencies, const int64_t* strides, int64_t tokens, int64_t n_q_heads,
+                                 int64_t n_kv_heads, int64_t head_dim, int64_t half, int64_t cache_slots,
+                                 int32_t interleaved, float factor, float key_scale, float value_scale, int32_t dtype,
+                                 int32_t cache_dtype, void* stream);
+
+/* out [sequences, n_q_heads, head_dim] of dtype: softmax(scale * key_scale * q . k) of the
+ * cached keys times value_scale times the values, query head h against key-value head
+ * h / (n_q_heads / n_kv_heads). q: one token a sequence. Caches [pages, page_size,
+ * n_kv_heads, head_dim] of dtype or FP8; position t of sequence b is at place t %
+ * page_size of page page_table[b][t / page_size]. Seen are the positions below
+ * lengths[b] (at most table_width * page_size, which is at most 2^30) and, with window >
+ * 0, the last `window` of them; positions on a page outside [0, pages) are left out.
+ * Where none is left, out is zeros and lse -infinity. lse [sequences, n_q_heads]: log of
+ * the sum of the exponentials, or NULL. head_dim: a multiple of 16, at most 256.
+ * workspace: cck_paged_attention_workspace(...) bytes, aligned to 16, for this call alone
+ * until it has run. */
+int32_t launch_paged_attention_fwd(const void* q, const void* key_cache, const void* value_cache,
+                                   const int64_t* page_table, const int64_t* lengths, void* out, float* lse,
+                                   void* workspace, int64_t q_token_stride, int64_t q_head_stride, int64_t sequences,
+                                   int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim, int64_t pages,
+                                   int64_t page_size, int64_t table_width, int64_t window, float scale,
+                                   float key_scale, float value_scale, int32_t dtype, int32_t cache_dtype,
+                                   void* stream);
+int64_t cck_paged_attention_workspace(int64_t sequences, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
+                                      int64_t page_size, int64_t table_width);
+
 /* ---- Diagnostics (no reference counterpart): device-side checks of the
  * arithmetic shortcuts used on the FP8 fast path. ---- */
 
