@@ -444,6 +444,26 @@ void fp8_quant_token_fwd(py::handle x, py::handle x_fp8, py::handle scale, const
                                           xv.dtype, fmt, st));
 }
 
+void fp8_quant_group_fwd(py::handle x, py::handle x_fp8, py::handle scale, const std::string& fmt_str) {
+  const int32_t fmt = parse_fp8_format(fmt_str);
+  View xv = validate_tensor("x", x);
+  View qv = validate_tensor("x_fp8", x_fp8);
+  View sv = validate_tensor("scale", scale);
+  check_fp8_common(xv, qv, fmt, fmt_str);
+  require_f32("scale", sv);
+  check_2d_and_codes(xv, qv);
+  const int64_t m = xv.shape[0], n = xv.shape[1];
+  if (sv.shape != std::vector<int64_t>{m, (n + 127) / 128}) {
+    shape_mismatch("scale shape " + shape_str(sv.shape) + " must be [" + std::to_string(m) + ", " +
+                   std::to_string((n + 127) / 128) + "] (M, ceil(N/128))");
+  }
+  if (n > INT32_MAX) shape_mismatch("rows of more than 2^31 - 1 elements");
+  const Launch launch(xv.device_index);
+  check_launch("launch_fp8_quant_group_fwd",
+               launch_fp8_quant_group_fwd((const void*)xv.ptr, (uint8_t*)qv.ptr, (float*)sv.ptr, m, n, xv.dtype, fmt,
+                                          launch.st));
+}
+
 // The float32 one-element tensor that receives a static scale (the scale
 // tensor the Python API returns), or nullptr for None.
 float* static_scale_out(py::handle scale_out) {
@@ -937,6 +957,69 @@ void mxfp4_linear_fwd(py::handle x_codes, py::handle x_scales, py::handle w_code
                                        rows, experts, n, blocks, yv.dtype, launch.st));
 }
 
+// FP8 codes.
+View validate_fp8(const char* name, const py::handle& obj) {
+  View v = validate_tensor(name, obj);
+  if (v.dtype != F8E4M3 && v.dtype != F8E5M2) {
+    value_error(std::string("unsupported dtype '") + tag_to_dtype_str(v.dtype) + "': " + name +
+                " must be float8_e4m3fn or float8_e5m2");
+  }
+  return v;
+}
+
+// x [rows, k] with scales [rows or ceil(rows / 128), ceil(k / 128)]; w [n, k] or with offsets
+// [num_experts, n, k], with scales [.., ceil(n / 128), ceil(k / 128)].
+void fp8_block_linear_fwd(py::handle x, py::handle x_scale, py::handle w, py::handle w_scale, py::handle offsets,
+                          py::handle y) {
+  View xv = validate_fp8("x_codes", x);
+  View xs = validate_tensor("x_scale", x_scale);
+  View wv = validate_fp8("w_codes", w);
+  View ws = validate_tensor("w_scale", w_scale);
+  std::optional<View> ov;
+  if (!offsets.is_none()) ov = validate_int64_tensor("offsets", offsets);
+  View yv = validate_tensor("y", y);
+  require_f32("x_scale", xs);
+  require_f32("w_scale", ws);
+  require_float("y", yv);
+  check_same_device("x_scale", xs, xv, "x_codes");
+  check_same_device("w_codes", wv, xv, "x_codes");
+  check_same_device("w_scale", ws, xv, "x_codes");
+  if (ov) check_same_device("offsets", *ov, xv, "x_codes");
+  check_same_device("y", yv, xv, "x_codes");
+  if (xv.shape.size() != 2) shape_mismatch("x_codes must be 2-D [rows, k], got " + shape_str(xv.shape));
+  const int64_t experts = ov ? check_offsets(*ov) : 1, rows = xv.shape[0], k = xv.shape[1], blocks = (k + 127) / 128;
+  const size_t dims = ov ? 3 : 2;
+  if (wv.shape.size() != dims || (ov && wv.shape[0] != experts) || wv.shape.back() != k) {
+    shape_mismatch(std::string("w_codes must be ") + (ov ? "[num_experts, n, k] with offsets [num_experts + 1]"
+                                                         : "[n, k] without offsets") +
+                   " and have x_codes' k; got x_codes=" + shape_str(xv.shape) + ", w_codes=" + shape_str(wv.shape));
+  }
+  const int64_t n = wv.shape[dims - 2];
+  const bool group = xs.shape == std::vector<int64_t>{rows, blocks};
+  if (!group && xs.shape != std::vector<int64_t>{(rows + 127) / 128, blocks}) {
+    shape_mismatch("x_scale shape " + shape_str(xs.shape) + " must be [" + std::to_string(rows) + ", " +
+                   std::to_string(blocks) + "] (\"group\") or [" + std::to_string((rows + 127) / 128) + ", " +
+                   std::to_string(blocks) + "] (\"block\")");
+  }
+  std::vector<int64_t> want = wv.shape;
+  want[dims - 2] = (n + 127) / 128;
+  want[dims - 1] = blocks;
+  if (ws.shape != want) {
+    shape_mismatch("w_scale shape " + shape_str(ws.shape) + " must be " + shape_str(want) + " (\"block\")");
+  }
+  if (yv.shape != std::vector<int64_t>{rows, n}) {
+    shape_mismatch("y shape " + shape_str(yv.shape) + " must be [" + std::to_string(rows) + ", " + std::to_string(n) +
+                   "]");
+  }
+  check_product_sizes(rows, n * dtype_bytes(yv.dtype), k);
+  const Launch launch(xv.device_index);
+  check_launch("launch_fp8_block_linear_fwd",
+               launch_fp8_block_linear_fwd((const void*)xv.ptr, (const float*)xs.ptr, (const void*)wv.ptr,
+                                           (const float*)ws.ptr, ov ? (const int64_t*)ov->ptr : nullptr, (void*)yv.ptr,
+                                           rows, experts, n, k, group ? 1 : 128, xv.dtype, wv.dtype, yv.dtype,
+                                           launch.st));
+}
+
 }  // namespace
 
 #include "native_decode.hpp"
@@ -982,6 +1065,10 @@ PYBIND11_MODULE(_native, m) {
   m.def("mxfp4_dequant_fwd", &mxfp4_dequant_fwd, py::arg("codes"), py::arg("scales"), py::arg("out"));
   m.def("mxfp4_linear_fwd", &mxfp4_linear_fwd, py::arg("x_codes"), py::arg("x_scales"), py::arg("w_codes"),
         py::arg("w_scales"), py::arg("offsets"), py::arg("y"));
+  m.def("fp8_quant_group_fwd", &fp8_quant_group_fwd, py::arg("x"), py::arg("x_fp8"), py::arg("scale"),
+        py::arg("fp8_format"));
+  m.def("fp8_block_linear_fwd", &fp8_block_linear_fwd, py::arg("x_codes"), py::arg("x_scale"), py::arg("w_codes"),
+        py::arg("w_scale"), py::arg("offsets"), py::arg("y"));
   m.def("rope_at_fwd", &rope_at_fwd, py::arg("q"), py::arg("k"), py::arg("positions"), py::arg("frequencies"),
         py::arg("q_out"), py::arg("k_out"), py::arg("layout"), py::arg("scale"), py::arg("inverse"));
   m.def("rope_to_cache_fwd", &rope_to_cache_fwd, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("key_cache"),

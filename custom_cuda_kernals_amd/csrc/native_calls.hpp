@@ -305,13 +305,15 @@ inline PyObject* fp8_quant(PyObject*, PyArgs a, Py_ssize_t n) {
   const bool block = PyUnicode_CompareWithASCIIString(a[2], "block") == 0;
   const bool token = !block && PyUnicode_CompareWithASCIIString(a[2], "token") == 0;
   const bool tensor = !block && !token && PyUnicode_CompareWithASCIIString(a[2], "tensor") == 0;
-  if (fmt < 0 || !x || float_tag(x) < 0 || x.dim() != 2 || !(block || token || tensor) || (is_static && !tensor)) {
+  const bool group = !block && !token && !tensor && PyUnicode_CompareWithASCIIString(a[2], "group") == 0;
+  if (fmt < 0 || !x || float_tag(x) < 0 || x.dim() != 2 || !(block || token || tensor || group) ||
+      (is_static && !tensor) || (group && x.size(1) > INT32_MAX)) {
     Py_RETURN_NONE;
   }
   const int64_t m = x.size(0), cols = x.size(1);
   const int32_t dt = float_tag(x);
-  const int64_t tiles[2] = {(m + 127) / 128, (cols + 127) / 128};
-  const c10::IntArrayRef scales = block ? c10::IntArrayRef(tiles) : token ? x.sizes().slice(0, 1) : c10::IntArrayRef(kOne);
+  const int64_t tiles[2] = {group ? m : (m + 127) / 128, (cols + 127) / 128};
+  const c10::IntArrayRef scales = block || group ? c10::IntArrayRef(tiles) : token ? x.sizes().slice(0, 1) : c10::IntArrayRef(kOne);
   const Launch launch(x.device().index());
   at::Tensor out[2];
   allocate(x.device(), {{x.sizes(), fp8_type(fmt)}, {scales, c10::ScalarType::Float}}, out);
@@ -322,6 +324,8 @@ inline PyObject* fp8_quant(PyObject*, PyArgs a, Py_ssize_t n) {
   if (is_static) {
     check_launch("launch_fp8_quant_static_fwd",
                  launch_fp8_quant_static_fwd(xp, qp, value, sp, m, cols, dt, fmt, launch.st));
+  } else if (group) {
+    check_launch("launch_fp8_quant_group_fwd", launch_fp8_quant_group_fwd(xp, qp, sp, m, cols, dt, fmt, launch.st));
   } else if (block) {
     check_launch("launch_fp8_quant_block_fwd", launch_fp8_quant_block_fwd(xp, qp, sp, m, cols, dt, fmt, launch.st));
   } else if (token) {
@@ -577,6 +581,42 @@ inline PyObject* mxfp4_linear(PyObject*, PyArgs a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// (x_codes, x_scale, w_codes, w_scale, offsets, out_dtype)
+inline PyObject* fp8_block_linear(PyObject*, PyArgs a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (n_args != 6 || !ordinary_state()) Py_RETURN_NONE;
+  const Input x(a[0]), xs(a[1]), w(a[2]), ws(a[3]);
+  const bool grouped = a[4] != Py_None;
+  const Input offsets(grouped ? a[4] : a[0]);
+  const int32_t dt = dtype_arg(a[5]);
+  const int64_t dims = grouped ? 3 : 2;
+  if (!x || !xs || !w || !ws || !offsets || dt < 0 || !is_fp8(tag_of(x.type())) || !is_fp8(tag_of(w.type())) ||
+      xs.type() != c10::ScalarType::Float || ws.type() != c10::ScalarType::Float || w.device() != x.device() ||
+      xs.device() != x.device() || ws.device() != x.device() || x.dim() != 2 || xs.dim() != 2 || w.dim() != dims ||
+      ws.dim() != dims || w.size(-1) != x.size(1)) {
+    Py_RETURN_NONE;
+  }
+  const int64_t experts = grouped ? offsets_experts(offsets, x) : 1;
+  const int64_t rows = x.size(0), k = x.size(1), n = w.size(-2), blocks = (k + 127) / 128;
+  if (experts == 0 || (grouped && (w.size(0) != experts || ws.size(0) != experts)) || ws.size(-1) != blocks ||
+      ws.size(-2) != (n + 127) / 128 || xs.size(1) != blocks || (xs.size(0) != rows && xs.size(0) != (rows + 127) / 128) ||
+      !product_sizes_ok(rows, n * dtype_bytes(dt), k)) {
+    Py_RETURN_NONE;
+  }
+  const int64_t sizes[2] = {rows, n};
+  const Launch launch(x.device().index());
+  at::Tensor out[1];
+  allocate(x.device(), {{sizes, reinterpret_cast<THPDtype*>(a[5])->scalar_type}}, out);
+  if (!unchanged(x, xs, w, ws, offsets)) Py_RETURN_NONE;
+  check_launch("launch_fp8_block_linear_fwd",
+               launch_fp8_block_linear_fwd(x.data(), (const float*)xs.data(), w.data(), (const float*)ws.data(),
+                                           grouped ? (const int64_t*)offsets.data() : nullptr, out[0].data_ptr(), rows,
+                                           experts, n, k, xs.size(0) == rows ? 1 : 128, tag_of(x.type()),
+                                           tag_of(w.type()), dt, launch.st));
+  return result(std::move(out[0]));
+  END_HANDLE_TH_ERRORS
+}
+
 // [..., heads, head_dim] as validate_heads takes it: its strides of tokens and heads.
 struct HeadsOf {
   int64_t tokens = 0, heads = 0, dim = 0, token_stride = 0, head_stride = 0;
@@ -785,6 +825,7 @@ inline PyMethodDef kMethods[] = {
     {"mxfp4_quant_call", as_method<mxfp4_quant>(), METH_FASTCALL, nullptr},
     {"mxfp4_dequant_call", as_method<mxfp4_dequant>(), METH_FASTCALL, nullptr},
     {"mxfp4_linear_call", as_method<mxfp4_linear>(), METH_FASTCALL, nullptr},
+    {"fp8_block_linear_call", as_method<fp8_block_linear>(), METH_FASTCALL, nullptr},
     {"rope_at_call", as_method<rope_at>(), METH_FASTCALL, nullptr},
     {"rope_to_cache_call", as_method<rope_to_cache>(), METH_FASTCALL, nullptr},
     {"paged_attention_call", as_method<paged_attention>(), METH_FASTCALL, nullptr},

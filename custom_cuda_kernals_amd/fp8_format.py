@@ -5,8 +5,8 @@ An FP8 activation is a pair ``(codes, scale)``:
 * ``codes``: ``[M, N]`` row-major, one byte per element, torch dtype
   ``float8_e4m3fn`` (OCP e4m3fn, as on gfx950; not MI300's fnuz) or
   ``float8_e5m2``. A code decodes exactly to an fp32 value ``c``.
-* ``scale``: float32, one of three layouts (the reference's two,
-  custom_cuda/kernels/fp8_quant.py:53-63, plus the per-token one):
+* ``scale``: float32, one of four layouts (the reference's two,
+  custom_cuda/kernels/fp8_quant.py:53-63, plus the per-token and the per-group one):
 
   ================  =============================  ===========================
   granularity       scale shape                    element (i, j) dequantises
@@ -14,6 +14,7 @@ An FP8 activation is a pair ``(codes, scale)``:
   ``"token"``       ``[M]``                        ``c[i, j] * scale[i]``
   ``"tensor"``      ``[1]`` (dynamic or static)    ``c[i, j] * scale[0]``
   ``"block"``       ``[ceil(M/128), ceil(N/128)]`` ``c[i, j] * scale[i//128, j//128]``
+  ``"group"``       ``[M, ceil(N/128)]``           ``c[i, j] * scale[i, j//128]``
   ================  =============================  ===========================
 
   and ``scale = clamp(amax / FP8_MAX, min=1e-12)`` over the row / tensor /
@@ -29,9 +30,9 @@ scale modes, probed on MI355X with torch 2.10:
   ``[N, K]`` quantised with ``granularity="token"`` has exactly this per-output-
   channel scale.
 
-There is no ``_scaled_mm`` mode for 128x128 tiles on this stack: block-scaled
-activations are dequantised (``dequantize``) or fed to a GEMM that applies tile
-scales itself. ``fp8_linear`` maps the layouts above onto ``_scaled_mm`` and
+There is no ``_scaled_mm`` mode for scales of 128 elements on this stack: activations in
+``"block"`` or ``"group"`` layout go to ``kernels.fp8_block_linear``, with weights in
+``"block"`` layout, or are dequantised (``dequantize``). ``fp8_linear`` maps the layouts above onto ``_scaled_mm`` and
 raises ``ValueError`` for the combinations it cannot express.
 """
 
@@ -45,7 +46,7 @@ __all__ = ["FP8_DTYPES", "GRANULARITIES", "TILE", "scale_shape", "check_pair", "
            "dequantize"]
 
 FP8_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
-GRANULARITIES = ("token", "tensor", "block")
+GRANULARITIES = ("token", "tensor", "block", "group")
 TILE = 128
 
 
@@ -57,6 +58,8 @@ def scale_shape(granularity: str, m: int, n: int) -> tuple[int, ...]:
         return (1,)
     if granularity == "block":
         return (math.ceil(m / TILE), math.ceil(n / TILE))
+    if granularity == "group":
+        return (m, math.ceil(n / TILE))
     raise ValueError(f"granularity must be one of {GRANULARITIES}, got {granularity!r}")
 
 
@@ -89,9 +92,9 @@ def scaled_mm_scale(scale: torch.Tensor, granularity: str, side: str) -> torch.T
         return scale.reshape(())
     if granularity == "token":
         return scale.view(-1, 1) if side == "a" else scale.view(1, -1)
-    if granularity == "block":
-        raise ValueError("torch._scaled_mm has no 128x128-tile scale mode on ROCm: dequantize block-scaled "
-                         "operands or use a GEMM that applies tile scales")
+    if granularity in ("block", "group"):
+        raise ValueError("torch._scaled_mm has no 128x128-tile scale mode on ROCm: use kernels.fp8_block_linear, "
+                         "or dequantize")
     raise ValueError(f"granularity must be one of {GRANULARITIES}, got {granularity!r}")
 
 
@@ -127,6 +130,8 @@ def dequantize(codes: torch.Tensor, scale: torch.Tensor, granularity: str,
         s = scale.view(-1, 1)
     elif granularity == "tensor":
         s = scale.view(1, 1)
+    elif granularity == "group":
+        s = scale.repeat_interleave(TILE, dim=1)[:, :codes.shape[1]]
     else:
         m, n = codes.shape
         s = scale.repeat_interleave(TILE, dim=0)[:m].repeat_interleave(TILE, dim=1)[:, :n]

@@ -1,7 +1,8 @@
 """Dynamic / static FP8 quantisation.
 
 Keeps the reference signature and defaults (custom_cuda/kernels/fp8_quant.py:28-63)
-and adds ``granularity="token"`` (one scale per row) and a static ``scale``.
+and adds ``granularity="token"`` (one scale per row), ``"group"`` (one for 128
+neighbours of a row) and a static ``scale``.
 Semantics: ``scale = clamp(amax / FP8_MAX, min=1e-12)``,
 ``x_fp8 = (x.float() / scale).to(fp8)`` (baselines/fp8_quant.py:162-189).
 """
@@ -38,8 +39,9 @@ def fp8_quant(
     """Quantise a ``[M, N]`` float32/float16/bfloat16 device tensor to FP8.
 
     ``granularity``: ``"block"`` (one scale per 128x128 tile, scale
-    ``[ceil(M/128), ceil(N/128)]``), ``"tensor"`` (one scale, ``[1]``) or
-    ``"token"`` (one scale per row, ``[M]``). ``scale``: a static per-tensor
+    ``[ceil(M/128), ceil(N/128)]``), ``"tensor"`` (one scale, ``[1]``),
+    ``"token"`` (one scale per row, ``[M]``) or ``"group"`` (one per 128 neighbours
+    of a row, ``[M, ceil(N/128)]``: what ``fp8_block_linear`` takes, as ``"block"``). ``scale``: a static per-tensor
     scale (requires ``granularity="tensor"``); returned as a ``[1]`` tensor.
     Returns ``(x_fp8, scale)``.
     """
@@ -48,8 +50,8 @@ def fp8_quant(
     if out is not None:
         return out
     check_fp8_format(fp8_format)
-    if granularity not in ("block", "tensor", "token"):
-        raise ValueError(f"granularity must be 'block', 'tensor' or 'token', got {granularity!r}")
+    if granularity not in ("block", "tensor", "token", "group"):
+        raise ValueError(f"granularity must be 'block', 'tensor', 'token' or 'group', got {granularity!r}")
     if scale is not None and granularity != "tensor":
         raise ValueError("a static scale is per-tensor: use granularity='tensor'")
 
@@ -76,6 +78,11 @@ def fp8_quant(
     if granularity == "token":
         scales = torch.empty(m, dtype=torch.float32, device=device)
         native.fp8_quant_token_fwd(x, x_fp8, scales, fp8_format)
+        return x_fp8, scales
+
+    if granularity == "group":
+        scales = torch.empty(m, math.ceil(n / _BLOCK_SIZE), dtype=torch.float32, device=device)
+        native.fp8_quant_group_fwd(x, x_fp8, scales, fp8_format)
         return x_fp8, scales
 
     # The reference zero-fills an int32 that receives the amax bits and then

@@ -312,6 +312,23 @@ int32_t launch_paged_attention_fwd(const void* q, const void* key_cache, const v
 int64_t cck_paged_attention_workspace(int64_t sequences, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
                                       int64_t page_size, int64_t table_width);
 
+/* ---- FP8 with a scale for each block of 128 (no reference counterpart) ---- */
+
+/* One scale for 128 neighbours of a row: scale [m, ceil(n / 128)], codes as the other
+ * granularities of x [m, n]. */
+int32_t launch_fp8_quant_group_fwd(const void* x, uint8_t* x_fp8, float* scale, int64_t m, int64_t n, int32_t dtype,
+                                   int32_t fp8_format, void* stream);
+
+/* y[s][j] = sum over k of x[s][k] w[e][j][k], y [rows, n] of dtype, of FP8 codes x [rows,
+ * k] and w [num_experts, n, k] times their scales: x_scale [ceil(rows / x_block_rows),
+ * ceil(k / 128)] with x_block_rows 1 or 128, w_scale [num_experts, ceil(n / 128), ceil(k /
+ * 128)]. Sums in float32, each block's times its scales. offsets as for the expert
+ * products, or NULL with num_experts == 1 for a dense product. Formats CCK_DTYPE_F8*. */
+int32_t launch_fp8_block_linear_fwd(const void* x, const float* x_scale, const void* w, const float* w_scale,
+                                    const int64_t* offsets, void* y, int64_t rows, int64_t num_experts, int64_t n,
+                                    int64_t k, int32_t x_block_rows, int32_t x_format, int32_t w_format, int32_t dtype,
+                                    void* stream);
+
 /* ---- Diagnostics (no reference counterpart): device-side checks of the
  * arithmetic shortcuts used on the FP8 fast path. ---- */
 

@@ -235,3 +235,106 @@ def test_the_planted_mistake_is_seen():
     off = np.abs(a - b)[3]
     assert (off > 2.0 ** -21 * 2 * np.abs(x).max() + 2.0 ** -8).any() and np.array_equal(a[:3], b[:3])
     assert ofp8.FP8_MAX["e4m3"] == 448.0
+
+
+def linear_args(**kw):
+    a = {"x": T(5, 300, dtype=E4M3), "xs": T(5, 3, dtype=F32), "w": T(200, 300, dtype=E4M3), "ws": T(2, 3, dtype=F32),
+         "offsets": None, "y": T(5, 200)}
+    return [{**a, **kw}[n] for n in a]
+
+
+GROUPED = {"w": T(4, 200, 300, dtype=E4M3), "ws": T(4, 2, 3, dtype=F32), "offsets": T(5, dtype=I64)}
+
+
+@pytest.mark.parametrize("match,kw", [
+    ("x_codes must be float8", {"x": T(5, 300)}),
+    ("w_codes must be float8", {"w": T(200, 300, dtype=F32)}),
+    ("x_scale must be float32", {"xs": T(5, 3)}),
+    ("w_scale must be float32", {"ws": T(2, 3)}),
+    ("unsupported dtype", {"y": T(5, 200, dtype=E4M3)}),
+    ("device mismatch: 'w_codes'", {"w": T(200, 300, dtype=E4M3, index=1)}),
+    ("must be contiguous", {"w": T(200, 300, dtype=E4M3, strides=(1, 200))}),
+    ("x_codes must be 2-D", {"x": T(1, 5, 300, dtype=E4M3)}),
+    ("w_codes must be", {"w": T(200, 301, dtype=E4M3)}),
+    ("w_codes must be", {"w": T(4, 200, 300, dtype=E4M3)}),
+    ("w_codes must be", {**GROUPED, "w": T(3, 200, 300, dtype=E4M3)}),
+    ("offsets must be int64", {**GROUPED, "offsets": T(5, dtype=torch.int32)}),
+    ("num_experts in", {**GROUPED, "offsets": T(1, dtype=I64)}),
+    ("x_scale shape", {"xs": T(5, 2, dtype=F32)}),
+    ("x_scale shape", {"xs": T(3, 3, dtype=F32)}),
+    ("w_scale shape", {"ws": T(200, 3, dtype=F32)}),
+    ("w_scale shape", {**GROUPED, "ws": T(2, 3, dtype=F32)}),
+    ("y shape", {"y": T(5, 201)}),
+    ("4 MiB", {"x": T(5, 1 << 23, dtype=E4M3), "xs": T(5, 1 << 16, dtype=F32), "w": T(200, 1 << 23, dtype=E4M3),
+               "ws": T(2, 1 << 16, dtype=F32)}),
+])
+def test_fp8_block_linear_refuses(match, kw):
+    raises(match, native.fp8_block_linear_fwd, *linear_args(**kw))
+
+
+def test_group_quant_refuses():
+    for match, args in (("scale shape", (T(5, 300), T(5, 300, dtype=E4M3), T(5, 2, dtype=F32), "e4m3")),
+                        ("x_fp8 shape", (T(5, 300), T(5, 299, dtype=E4M3), T(5, 3, dtype=F32), "e4m3")),
+                        ("x must be 2-D", (T(300), T(300, dtype=E4M3), T(3, dtype=F32), "e4m3")),
+                        ("fp8_format", (T(5, 300), T(5, 300, dtype=E4M3), T(5, 3, dtype=F32), "e3m4"))):
+        raises(match, native.fp8_quant_group_fwd, *args)
+    raises("static scale is per-tensor", K.fp8_quant, torch.zeros(2, 128), "e4m3", "group", 0.5)
+    raises("must be a CUDA tensor", K.fp8_quant, torch.zeros(2, 128), "e4m3", "group")
+
+
+def test_the_python_linear_refuses_cpu_tensors():
+    x, w = torch.zeros(5, 128).to(E4M3), torch.zeros(7, 128).to(E4M3)
+    raises("must be a CUDA tensor", K.fp8_block_linear, x, torch.ones(5, 1), w, torch.ones(1, 1))
+    raises("x_codes must be 2-D", K.fp8_block_linear, x[0], torch.ones(1), w, torch.ones(1, 1))
+    raises("w_codes 3-D", K.fp8_block_linear, x, torch.ones(5, 1), w, torch.ones(1, 1), torch.zeros(2, dtype=I64))
+    args = (x, torch.ones(5, 1), w, torch.ones(1, 1), None, BF16)
+    for i in range(len(args)):
+        for other in (None, object(), 3, 2.5, "e4m3", 1 << 80, [1]):
+            assert native.fp8_block_linear_call(*args[:i], other, *args[i + 1:]) is None
+
+
+def test_launchers_refuse_and_take_nothing():
+    """Through the C ABI: 0 for no work, hipErrorInvalidValue (1) for sizes, tags and scales out of range,
+    both before any device call."""
+    import ctypes
+
+    from tests import _cck
+
+    lib, p, strides = _cck.load(), 1 << 20, (ctypes.c_int64 * 8)(*[64] * 8)
+    s = ctypes.cast(strides, ctypes.c_void_p)
+
+    def rope(tokens=1, dim=64, half=32, dtype=2):
+        return lib.launch_rope_at_fwd(p, p, p, p, p, p, s, tokens, 1, 1, dim, half, 0, 0, 1.0, dtype, None)
+
+    assert rope(tokens=0) == 0 and rope(dim=0) == 0
+    assert rope(dtype=3) == 1 and rope(half=33) == 1 and rope(half=-1) == 1 and rope(dim=4096) == 1
+
+    def cache(tokens=1, key_scale=1.0, cache_dtype=3, half=32):
+        return lib.launch_rope_to_cache_fwd(p, p, p, p, p, p, p, p, p, s, tokens, 1, 1, 64, half, 16, 0, 1.0, key_scale,
+                                            1.0, 2, cache_dtype, None)
+
+    assert cache(tokens=0) == 0
+    assert cache(key_scale=0.0) == 1 and cache(key_scale=math.inf) == 1 and cache(cache_dtype=1) == 1 and cache(half=40) == 1
+
+    def attention(sequences=1, heads=8, kv=2, dim=64, page=16, width=4, dtype=2, cache_dtype=2, workspace=None):
+        return lib.launch_paged_attention_fwd(p, p, p, p, p, p, None, workspace, 512, 64, sequences, heads, kv, dim, 9, page,
+                                              width, 0, 1.0, 1.0, 1.0, dtype, cache_dtype, None)
+
+    assert attention(sequences=0) == 0 and attention(heads=0) == 0
+    for bad in ({"heads": 7}, {"kv": 0}, {"dim": 72}, {"dim": 272}, {"page": 0}, {"width": -1}, {"width": 1 << 27},
+                {"dtype": 3}, {"cache_dtype": 1}, {"width": 400}, {"width": 400, "workspace": p + 4},
+                {"sequences": 1 << 23}):
+        assert attention(**bad) == 1, bad
+    room = lib.cck_paged_attention_workspace
+    room.restype, room.argtypes = ctypes.c_int64, [ctypes.c_int64] * 6
+    assert room(1, 8, 2, 64, 16, 4) == 0 and room(1, 8, 2, 64, 16, 400) > 0 and room(1, 7, 2, 64, 16, 400) == 0
+
+    def linear(rows=1, experts=1, n=16, k=128, block_rows=1, fx=3, fw=3, dtype=2):
+        return lib.launch_fp8_block_linear_fwd(p, p, p, p, None, p, rows, experts, n, k, block_rows, fx, fw, dtype, None)
+
+    assert linear(rows=0) == 0 and linear(n=0) == 0
+    for bad in ({"experts": 2}, {"block_rows": 64}, {"fx": 2}, {"fw": 0}, {"dtype": 3}, {"k": 1 << 23}, {"rows": 1 << 31}):
+        assert linear(**bad) == 1, bad
+    assert lib.launch_fp8_quant_group_fwd(p, p, p, 0, 5, 2, 3, None) == 0
+    assert lib.launch_fp8_quant_group_fwd(p, p, p, 1, 1 << 31, 2, 3, None) == 1
+    assert lib.launch_fp8_quant_group_fwd(p, p, p, 1, 5, 2, 2, None) == 1
