@@ -774,7 +774,7 @@ inline PyObject* paged_attention(PyObject*, PyArgs a, Py_ssize_t n) {
       table.type() != c10::ScalarType::Long || table.device() != q.device() || table.dim() != 2 ||
       table.size(0) != qh.tokens || !cache_scale_ok(key_scale, is_fp8(tag)) ||
       !cache_scale_ok(value_scale, is_fp8(tag)) ||
-      attention_limits(qh.tokens, qh.heads, kv, qh.dim, page, width) != nullptr) {
+      attention_limits(qh.tokens, qh.heads, kv, qh.dim, keys.size(0), page, width) != nullptr) {
     Py_RETURN_NONE;
   }
   const int64_t stats[2] = {qh.tokens, qh.heads};

@@ -216,10 +216,11 @@ void rope_to_cache_fwd(py::handle q, py::handle k, py::handle v, py::handle key_
 constexpr int64_t kMaxPositions = int64_t(1) << 30;
 
 // Limits of the attention's launcher that no shape check covers; nullptr if they hold.
-const char* attention_limits(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page,
-                             int64_t table_width) {
+const char* attention_limits(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, int64_t pages,
+                             int64_t page, int64_t table_width) {
   if (kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0) return "q's heads must be a multiple of the caches'";
   if (dim < 16 || dim > 256 || dim % 16 != 0) return "head_dim must be a multiple of 16, at most 256";
+  if (pages > INT32_MAX / page) return "a cache of 2^31 positions or more";
   if (table_width > kMaxPositions / page) return "page_table holds more than 2^30 positions a sequence";
   if (heads > 65536 || sequences > (int64_t(1) << 23) / heads) return "more than 2^23 query heads";
   return nullptr;
@@ -247,7 +248,8 @@ void paged_attention_fwd(py::handle q, py::handle key_cache, py::handle value_ca
     shape_mismatch("lengths shape " + shape_str(lv.shape) + " must be [" + std::to_string(qv.tokens) + "]");
   }
   if (window < 0) value_error("window must be 0 (none) or more, got " + std::to_string(window));
-  if (const char* wrong = attention_limits(qv.tokens, qv.heads, kv_heads, qv.dim, kc.shape[1], tv.shape[1])) {
+  if (const char* wrong = attention_limits(qv.tokens, qv.heads, kv_heads, qv.dim, kc.shape[0], kc.shape[1],
+                                          tv.shape[1])) {
     shape_mismatch(std::string(wrong) + "; got q=" + shape_str(qv.v.shape) + ", key_cache=" + shape_str(kc.shape) +
                    ", page_table=" + shape_str(tv.shape));
   }

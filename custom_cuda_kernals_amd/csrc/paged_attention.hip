@@ -15,17 +15,20 @@
 // one product to the other inside the lane. 16-bit P is split in two parts, high and low:
 // rounded once, it would add an error as large as that of the output's own rounding.
 //
-// Bound by HBM: reading keys and values once. A sequence is cut into as many parts as fill
-// the card; a workgroup takes a part of one key-value head, its four waves every fourth
-// step of it, each on its own until the sums of the waves meet in LDS. The parts' sums
-// meet in a second launch.
+// Bound by HBM: reading keys and values once. A sequence is cut into parts for as many
+// waves as fill the card; a workgroup is one wave with one part of one key-value head, and
+// the parts' sums meet in a second launch. Keys and values go straight from memory to LDS,
+// whole rows at a time, into a ring of two steps: a step is on its way while the one
+// before is worked on, without registers or other waves to wait for.
 #include "tile_product.hpp"
 
 namespace cck {
 namespace {
 
-constexpr int kWaves = 4, kHeads = 16;  // of a workgroup: waves, and query heads at most
-constexpr int kMinPart = 128;           // positions of a part, at least: a step of each wave
+constexpr int kHeads = 16;    // query heads of a workgroup, at most
+constexpr int kMinPart = 32;  // positions of a part, at least: a step
+constexpr int kFound = 512;   // positions whose slots are looked up at a time
+constexpr int kDepth = 2;     // steps in LDS
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Sums are scaled to a new maximum only where it is this much (a power of two) above the
 // one that they have.
@@ -42,6 +45,8 @@ struct AttentionArgs {
   int page_shift;
   float score_scale, value_scale;  // score_scale: with log2(e)
 };
+
+using i32x2 = int __attribute__((ext_vector_type(2)));
 
 // What the elements of a head's row are computed in. A chunk is what a lane loads of a
 // row: 16 bytes.
@@ -77,23 +82,31 @@ struct AsIs {
 template <class T, int FMT>
 struct FromCodes {
   static constexpr int kFragments = T::kBytes, kBytes = 1;
-  __device__ static f32x2 two(uint32_t w, bool high) {
-    if constexpr (FMT == kF8E4M3) {
-      return high ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  // Four codes to four elements, of 16 or 32 bits.
+  __device__ static void four(uint32_t w, uint32_t (&e)[T::kBytes]) {
+    if constexpr (T::kBytes == 4) {
+      const f32x2 a = FMT == kF8E4M3 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false) : __builtin_amdgcn_cvt_pk_f32_bf8((int)w, false);
+      const f32x2 b = FMT == kF8E4M3 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_bf8((int)w, true);
+      e[0] = f32_bits(a[0]), e[1] = f32_bits(a[1]), e[2] = f32_bits(b[0]), e[3] = f32_bits(b[1]);
+    } else if constexpr (std::is_same_v<T, Bf16>) {
+      e[0] = __builtin_bit_cast(uint32_t, FMT == kF8E4M3 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)
+                                                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, false));
+      e[1] = __builtin_bit_cast(uint32_t, FMT == kF8E4M3 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
+                                                         : __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, true));
     } else {
-      return high ? __builtin_amdgcn_cvt_pk_f32_bf8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_bf8((int)w, false);
+      e[0] = __builtin_bit_cast(uint32_t, FMT == kF8E4M3 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)
+                                                         : __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, 1.0f, false));
+      e[1] = __builtin_bit_cast(uint32_t, FMT == kF8E4M3 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true)
+                                                         : __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, 1.0f, true));
     }
   }
   __device__ static void fragments(const u32x4& w, u32x4 (&f)[kFragments]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const f32x2 a = two(w[i], false), b = two(w[i], true);
-      if constexpr (T::kBytes == 2) {
-        f[i / 2][i % 2 * 2] = T::pack(a[0], a[1]);
-        f[i / 2][i % 2 * 2 + 1] = T::pack(b[0], b[1]);
-      } else {
-        f[i] = (u32x4){f32_bits(a[0]), f32_bits(a[1]), f32_bits(b[0]), f32_bits(b[1])};
-      }
+      uint32_t e[T::kBytes];
+      four(w[i], e);
+#pragma unroll
+      for (int j = 0; j < T::kBytes; ++j) f[(i * T::kBytes + j) / 4][(i * T::kBytes + j) % 4] = e[j];
     }
   }
 };
@@ -117,28 +130,69 @@ struct Span {
   }
 };
 
-// LDS bytes of a row of values: an odd multiple of 32, so that eight rows begin in
-// different banks.
-constexpr __host__ __device__ int row_bytes(int elements, int bytes) { return ((elements * bytes + 31) / 32 | 1) * 32; }
-
-// DIM: the head's elements, padded. A step: kStep positions of a wave.
+// DIM: the head's elements, padded. A step: kStep positions. A row in LDS: kChunks of 16
+// bytes, chunk c at place c ^ key_place (or value_place) of its row, so that lanes that
+// read at the same time reach different banks.
 template <class T, class S, int DIM>
 struct Shape {
-  static constexpr int kTiles = T::kBytes == 4 ? 1 : 2, kStep = 16 * kTiles;
-  static constexpr int kElements = 16 / S::kBytes;             // of a chunk
-  static constexpr int kChunks = (DIM + 4 * kElements - 1) / (4 * kElements);  // of a lane and row
-  static constexpr int kRow = row_bytes(DIM, T::kBytes);
-  static constexpr int kWaveLds = kStep * kRow;
-  static constexpr int kSumsLds = kHeads * DIM * 4;
-  static constexpr int kLds = kWaves * (kWaveLds > kSumsLds ? kWaveLds : kSumsLds);
+  static constexpr int kTiles = S::kBytes == 4 ? 1 : 2, kStep = 16 * kTiles;
+  static constexpr int kElements = 16 / S::kBytes;       // of a chunk
+  static constexpr int kChunks = DIM / kElements;        // of a row
+  static constexpr int kOfLane = kChunks / 4;            // of a row, of a lane of the first product
+  static constexpr int kRow = DIM * S::kBytes;
+  static constexpr int kRows = 64 / kChunks;             // that one load instruction brings
+  static constexpr int kLoads = kStep / kRows;           // of a step, of keys or of values
+  static constexpr int kKeys = kStep * kRow, kSlot = 2 * kKeys;
+  static_assert(kChunks % 4 == 0 && kRows >= 1 && kRows <= 16 && 2 * kLoads < 64);
+  // A lane reads a chunk of one of 16 neighbouring rows.
+  __device__ static int key_place(int r) { return kChunks >= 8 ? r & 7 : (r ^ (r >> 2)) & 3; }
+  // 16-bit: 32 bytes of each of four neighbouring rows. FP8: 16 of four and of the four 16 rows on. fp32: 64 of
+  // each of four rows that are four apart.
+  __device__ static int value_place(int r) {
+    if constexpr (S::kBytes == 4) return ((r >> 2) & 3) << 2;
+    if constexpr (S::kBytes == 2) return kChunks >= 16 ? (r & 3) << 1 : ((r >> 1) & 1) << 1;
+    if constexpr (kChunks >= 16) return (r & 3) | ((r >> 4) & 1) << 2;
+    return kChunks == 8 ? ((r >> 1) & 1) | ((r >> 4) & 1) << 1 : (r >> 4) & 1;
+  }
 };
 
+// Four elements, eight or sixteen bytes, at any alignment.
+template <class C>
+__device__ inline void store4(const f32x4& v, char* p) {
+  float f[C::VEC] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = v[i];
+  const u32x4 w = C::pack(f);
+  if constexpr (C::kBytes == 4) {
+    *reinterpret_cast<u32x4_any*>(p) = w;
+  } else {
+    *reinterpret_cast<u32x2_any*>(p) = (u32x2){w[0], w[1]};
+  }
+}
+
+// 16 bytes per lane from p to LDS at the named place + 16 x lane (see lds_place).
+__device__ inline void load_to_place_from(const char* p) {
+  asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(p) : "memory");
+}
+
+// FP8 values of element 16 f + col and eight positions, 4 g .. 4 g + 3 and 16 on: lanes 2 j
+// and 2 j + 1 of 16 point at 16 codes of the j-th of eight rows, and lane i receives the
+// eight rows' i-th codes.
+template <class Sh>
+__device__ inline u32x2 codes_at(LdsPtr from, int f, int g, int col) {
+  using Lds2 = __attribute__((address_space(3))) i32x2*;
+  const int j = col >> 1, r = (j >> 2) * 16 + 4 * g + (j & 3);
+  const LdsPtr p = from + r * Sh::kRow + ((f ^ Sh::value_place(r)) << 4) + (col & 1) * 8;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<Lds2>(p)));
+}
+
 template <class T, class S, int DIM>
-__global__ __launch_bounds__(kWaves * 64, T::kBytes == 2 && DIM <= 128 ? 2 : 1) void paged_attention(AttentionArgs a) {
+__global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
   using Sh = Shape<T, S, DIM>;
-  constexpr int kTiles = Sh::kTiles, kStep = Sh::kStep, kChunks = Sh::kChunks, kFrags = S::kFragments, kRow = Sh::kRow;
-  __shared__ __attribute__((aligned(64))) char lds[Sh::kLds];
-  __shared__ float stats[kWaves][kHeads][2];
+  constexpr int kTiles = Sh::kTiles, kStep = Sh::kStep, kOfLane = Sh::kOfLane, kFrags = S::kFragments;
+  constexpr int kRow = Sh::kRow, kAll = 2 * Sh::kLoads;
+  __shared__ __attribute__((aligned(1024))) char lds[kDepth * Sh::kSlot];
+  __shared__ int found[kFound];
 
   const int units = a.kv_heads * a.head_tiles;
   int id = blockIdx.x;
@@ -150,17 +204,16 @@ __global__ __launch_bounds__(kWaves * 64, T::kBytes == 2 && DIM <= 128 ? 2 : 1) 
   const Span span(a, sequence, part);
   if (part >= span.count && part > 0) return;
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int col = lane & 15, g = lane >> 4;
-  const LdsPtr mine = (LdsPtr)lds + wave * Sh::kWaveLds;
+  const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
+  const int row_bytes = a.dim * S::kBytes;
 
   // The columns' queries: of each chunk of a row the elements that this lane has.
-  u32x4 q[kChunks][kFrags];
+  u32x4 q[kOfLane][kFrags];
   {
     const int h = kv * group + head0 + (col < heads ? col : 0);
     const char* from = a.q + ((int64_t)sequence * a.q_token + (int64_t)h * a.q_head) * T::kBytes;
 #pragma unroll
-    for (int s = 0; s < kChunks; ++s) {
+    for (int s = 0; s < kOfLane; ++s) {
 #pragma unroll
       for (int f = 0; f < kFrags; ++f) {
         const int e = (4 * s + g) * Sh::kElements + f * (16 / T::kBytes);
@@ -170,94 +223,117 @@ __global__ __launch_bounds__(kWaves * 64, T::kBytes == 2 && DIM <= 128 ? 2 : 1) 
     }
   }
 
+  // They are here before the loop: a wait of the compiler's inside it would be one for the steps on their way too.
+#pragma unroll
+  for (int s = 0; s < kOfLane; ++s) {
+#pragma unroll
+    for (int f = 0; f < kFrags; ++f) asm volatile("" : "+v"(q[s][f]));
+  }
+
+  // Slots of the positions from `first` on, kFound of them; -1 for none.
   const int64_t* table = a.table + (int64_t)sequence * a.table_width;
-  const int64_t slot_bytes = (int64_t)a.kv_heads * a.dim * S::kBytes;
-  const int64_t head_bytes = (int64_t)kv * a.dim * S::kBytes;
-  // Where the lane's positions of a step lie: slots, or -1 for none.
-  auto find = [&](int first, int64_t (&slot)[kTiles]) __attribute__((always_inline)) {
+  auto find = [&](int first, auto each) __attribute__((always_inline)) {
+    constexpr int kEach = decltype(each)::value;  // of a lane
+    int64_t page[kEach];
+    int in_page[kEach];
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      const int t = first + 16 * j + col;
-      slot[j] = -1;
-      if (t < span.end) {
-        const uint32_t at = (uint32_t)(((uint64_t)(uint32_t)t * a.page_magic) >> a.page_shift);
-        const int64_t page = table[at];
-        if (page >= 0 && page < a.pages) slot[j] = page * a.page + (t - (int)at * a.page);
-      }
+    for (int i = 0; i < kEach; ++i) {
+      const int t = first + i * 64 + lane, last = span.end - 1;
+      const uint32_t u = (uint32_t)(t < last ? t : last);
+      const uint32_t at = (uint32_t)(((uint64_t)u * a.page_magic) >> a.page_shift);
+      page[i] = table[at];
+      in_page[i] = (int)(u - at * (uint32_t)a.page);
     }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const bool there = first + i * 64 + lane < span.end && page[i] >= 0 && page[i] < a.pages;
+      found[i * 64 + lane] = there ? (int)page[i] * a.page + in_page[i] : -1;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
   };
-  const int row = a.dim * S::kBytes;
-  u32x4 k[kTiles][kChunks], v[kTiles][kChunks];
-  auto load = [&](const int64_t (&slot)[kTiles]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      const int64_t at = (slot[j] < 0 ? 0 : slot[j]) * slot_bytes + head_bytes;
-#pragma unroll
-      for (int s = 0; s < kChunks; ++s) {
-        const int byte = (4 * s + g) * 16, last = row - 16;  // past the row its last chunk will do
-        k[j][s] = *reinterpret_cast<const u32x4_any*>(a.keys + at + (byte < last ? byte : last));
-        v[j][s] = *reinterpret_cast<const u32x4_any*>(a.values + at + (byte < last ? byte : last));
+  // The lane's row and chunk of a load instruction's kRows rows.
+  const int load_row = lane / Sh::kChunks, load_chunk = lane % Sh::kChunks;
+  const int64_t slot_bytes = (int64_t)a.kv_heads * row_bytes;
+  const char *const keys = a.keys + (int64_t)kv * row_bytes, *const values = a.values + (int64_t)kv * row_bytes;
+  // Asks for a step of keys and values; which of its positions there are.
+  auto ask = [&](int first, LdsPtr to) __attribute__((always_inline)) {
+    const int at = first - span.begin;
+    if (at % kFound == 0) {
+      if (span.end - first <= 64) {
+        find(first, IntC<1>{});
+      } else {
+        find(first, IntC<kFound / 64>{});
       }
     }
+    const int mine = found[at % kFound + (lane & (kStep - 1))];
+#pragma unroll
+    for (int i = 0; i < Sh::kLoads; ++i) {
+      const int r = i * Sh::kRows + load_row;
+      const int slot = found[at % kFound + r];
+      // past the row its last chunk will do, and for a position that is not there any row
+      const int key_byte = (load_chunk ^ Sh::key_place(r)) * 16, value_byte = (load_chunk ^ Sh::value_place(r)) * 16;
+      const int64_t row = (int64_t)(uint32_t)(slot < 0 ? 0 : slot) * slot_bytes;
+      lds_place(to + i * 1024);
+      place_ready();
+      load_to_place_from(keys + (row + (key_byte < row_bytes ? key_byte : row_bytes - 16)));
+      lds_place(to + Sh::kKeys + i * 1024);
+      place_ready();
+      load_to_place_from(values + (row + (value_byte < row_bytes ? value_byte : row_bytes - 16)));
+    }
+    return (uint32_t)__ballot(mine >= 0);
   };
 
   constexpr int kOut = DIM / 16;
   f32x4 out[kOut] = {};
   float top = -__builtin_inff(), base = 0.0f, sum = 0.0f;  // base: top, or 0 while there is none
-  int64_t slot[kTiles], next_slot[kTiles];
-  int first = span.begin + wave * kStep;
-  find(first, slot);
-  if (first < span.end) load(slot);
-  find(first + kWaves * kStep, next_slot);
-  for (; first < span.end; first += kWaves * kStep) {
-    // Values to LDS, those of positions that are not seen as zeros.
-    uint64_t seen[kTiles];
-    bool all = true;
+  auto step = [&](const LdsPtr slot, uint32_t seen) __attribute__((always_inline)) {
+    constexpr uint32_t kEvery = kStep == 32 ? 0xffffffffu : 0xffffu;
+    const bool all = (seen & kEvery) == kEvery;
+    u32x4 k[kTiles][kOfLane];
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      seen[j] = __ballot(slot[j] >= 0);
-      all = all && seen[j] == ~0ull;
+    for (int s = 0; s < kOfLane; ++s) {
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j) {
+        k[j][s] = lds_load<u32x4>(slot + (16 * j + col) * kRow + (((4 * s + g) ^ Sh::key_place(col)) << 4));
+      }
     }
+    if (row_bytes < kRow) {  // there is more in LDS than the row
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
+      for (int s = 0; s < kOfLane; ++s) {
 #pragma unroll
-      for (int s = 0; s < kChunks; ++s) {
-        u32x4 w = v[j][s];
-        if (!all && slot[j] < 0) w = (u32x4){0u, 0u, 0u, 0u};
-        u32x4 f[kFrags];
-        S::fragments(w, f);
-        const int e = (4 * s + g) * Sh::kElements;
-        if (DIM % (4 * Sh::kElements) == 0 || e < DIM) {
-#pragma unroll
-          for (int i = 0; i < kFrags; ++i) lds_store(f[i], mine + (16 * j + col) * kRow + e * T::kBytes + i * 16);
+        for (int j = 0; j < kTiles; ++j) {
+          if ((4 * s + g) * 16 >= row_bytes) k[j][s] = (u32x4){0u, 0u, 0u, 0u};
         }
       }
     }
     f32x4 score[kTiles] = {};
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
+    for (int s = 0; s < kOfLane; ++s) {
 #pragma unroll
-      for (int s = 0; s < kChunks; ++s) {
-        u32x4 w = k[j][s], f[kFrags];
-        if ((4 * s + 4) * 16 > row && (4 * s + g) * 16 >= row) w = (u32x4){0u, 0u, 0u, 0u};
-        S::fragments(w, f);
+      for (int j = 0; j < kTiles; ++j) {
+        u32x4 f[kFrags];
+        S::fragments(k[j][s], f);
 #pragma unroll
         for (int i = 0; i < kFrags; ++i) score[j] = T::mma(f[i], q[s][i], score[j]);
       }
     }
-    // The next step's.
-#pragma unroll
-    for (int j = 0; j < kTiles; ++j) slot[j] = next_slot[j];
-    if (first + kWaves * kStep < span.end) load(slot);
-    find(first + 2 * kWaves * kStep, next_slot);
-
+    const LdsPtr from = slot + Sh::kKeys;
+    if (!all) {  // values that are not seen may be anything: zeros
+      const u32x4 zeros = {0u, 0u, 0u, 0u};
+      for (int i = 0; i < Sh::kLoads; ++i) {
+        if (!(seen >> (i * Sh::kRows + load_row) & 1)) lds_store(zeros, from + i * 1024 + lane * 16);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
     float most = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float x = score[j][i] * a.score_scale;
-        if (!all && !(seen[j] >> (4 * g + i) & 1)) x = -__builtin_inff();
+        if (!all && !(seen >> (16 * j + 4 * g + i) & 1)) x = -__builtin_inff();
         score[j][i] = x;
         most = __builtin_fmaxf(most, x);
       }
@@ -281,8 +357,7 @@ __global__ __launch_bounds__(kWaves * 64, T::kBytes == 2 && DIM <= 128 ? 2 : 1) 
         sum += score[j][i];
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    // Elements past the head's are computed with what is in LDS there, and not stored.
     if constexpr (T::kBytes == 2) {
       u32x4 high, low;
 #pragma unroll
@@ -295,82 +370,104 @@ __global__ __launch_bounds__(kWaves * 64, T::kBytes == 2 && DIM <= 128 ? 2 : 1) 
           low[2 * j + i] = T::pack(x - T::low(h), y - T::high(h));
         }
       }
-      // Four rows of 16 elements, turned over: row 4 g + lane / 4 % 4 of a tile.
-      using Lds4 = __attribute__((address_space(3))) s16x4*;
-      const LdsPtr from = mine + (4 * g + (col >> 2)) * kRow + (col & 3) * 8;
 #pragma unroll
       for (int f = 0; f < kOut; ++f) {
-        if (16 * f < a.dim) {
-          const u32x2 x = __builtin_bit_cast(
-              u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<Lds4>(from + f * 32)));
-          const u32x2 y = __builtin_bit_cast(
-              u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<Lds4>(from + f * 32 + 16 * kRow)));
-          const u32x4 w = {x[0], x[1], y[0], y[1]};
-          out[f] = T::mma(w, high, out[f]);
-          out[f] = T::mma(w, low, out[f]);
+        u32x4 w;
+        if constexpr (S::kBytes == 2) {
+          // Four rows of 16 elements, turned over: row 4 g + col / 4 of a tile, and 16 on, which has the same place.
+          using Lds4 = __attribute__((address_space(3))) s16x4*;
+          const int r = 4 * g + (col >> 2), c = (2 * f + ((col >> 1) & 1)) ^ Sh::value_place(r);
+          const LdsPtr p = from + r * kRow + c * 16 + (col & 1) * 8;
+          const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<Lds4>(p)));
+          const u32x2 y =
+              __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<Lds4>(p + 16 * kRow)));
+          w = (u32x4){x[0], x[1], y[0], y[1]};
+        } else {
+          uint32_t e[2], e2[2];
+          const u32x2 x = codes_at<Sh>(from, f, g, col);
+          S::four(x[0], e);
+          S::four(x[1], e2);
+          w = (u32x4){e[0], e[1], e2[0], e2[1]};
         }
+        out[f] = T::mma(w, high, out[f]);
+        out[f] = T::mma(w, low, out[f]);
       }
     } else {
-      const u32x4 p = __builtin_bit_cast(u32x4, score[0]);
 #pragma unroll
       for (int f = 0; f < kOut; ++f) {
-        if (16 * f < a.dim) {
+        if constexpr (S::kBytes == 4) {
           u32x4 w;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = lds_load<uint32_t>(mine + (4 * g + i) * kRow + (16 * f + col) * 4);
-          out[f] = T::mma(w, p, out[f]);
+          for (int i = 0; i < 4; ++i) {
+            const int r = 4 * g + i, c = (4 * f + (col >> 2)) ^ Sh::value_place(r);
+            w[i] = lds_load<uint32_t>(from + r * kRow + c * 16 + (col & 3) * 4);
+          }
+          out[f] = T::mma(w, __builtin_bit_cast(u32x4, score[0]), out[f]);
+        } else {
+          const u32x2 x = codes_at<Sh>(from, f, g, col);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t e[4];
+            S::four(x[j], e);
+            out[f] = T::mma((u32x4){e[0], e[1], e[2], e[3]}, __builtin_bit_cast(u32x4, score[j]), out[f]);
+          }
         }
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+  };
+
+  const LdsPtr slots = (LdsPtr)lds;
+  const int begin = span.begin, end = span.end;
+  uint32_t seen[kDepth] = {};
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) {
+    if (begin + d * kStep < end) seen[d] = ask(begin + d * kStep, slots + d * Sh::kSlot);
+  }
+  for (int first = begin; first < end; first += kDepth * kStep) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      const int now = first + d * kStep;
+      if (now < end) {
+        if (now + kStep < end) {
+          loads_landed<(kDepth - 1) * kAll>();
+        } else {
+          loads_landed();
+        }
+        step(slots + d * Sh::kSlot, seen[d]);
+        if (now + kDepth * kStep < end) {
+          lds_read();
+          seen[d] = ask(now + kDepth * kStep, slots + d * Sh::kSlot);
+        }
+      }
+    }
   }
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
 
-  // The waves' sums meet: [wave][head][dim] in LDS.
-  __syncthreads();
-  float* const sums = reinterpret_cast<float*>(lds);
-  if (g == 0) {
-    stats[wave][col][0] = top;
-    stats[wave][col][1] = sum;
-  }
+  if (col >= heads) return;
+  const int64_t head = (int64_t)sequence * a.heads + kv * group + head0 + col;
+  if (a.parts > 1) {
+    const int64_t at = head * a.parts + part;
 #pragma unroll
-  for (int f = 0; f < kOut; ++f) {
-    *reinterpret_cast<f32x4*>(sums + (wave * kHeads + col) * DIM + 16 * f + 4 * g) = out[f];
-  }
-  __syncthreads();
-  const int quads = a.dim / 4;
-  for (int i = threadIdx.x; i < heads * quads; i += kWaves * 64) {
-    const int h = i / quads, d = (i - h * quads) * 4;
-    float all_top = stats[0][h][0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) all_top = __builtin_fmaxf(all_top, stats[w][h][0]);
-    const float all_base = all_top == -__builtin_inff() ? 0.0f : all_top;
-    float total = 0.0f;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float weight = __builtin_amdgcn_exp2f(stats[w][h][0] - all_base);
-      total += weight * stats[w][h][1];
-      o += weight * *reinterpret_cast<const f32x4*>(sums + (w * kHeads + h) * DIM + d);
+    for (int f = 0; f < kOut; ++f) {
+      if (16 * f < a.dim) *reinterpret_cast<f32x4*>(a.partial + at * a.dim + 16 * f + 4 * g) = out[f];
     }
-    const int64_t head = (int64_t)sequence * a.heads + kv * group + head0 + h;
-    if (a.parts > 1) {
-      const int64_t row = head * a.parts + part;
-      *reinterpret_cast<f32x4*>(a.partial + row * a.dim + d) = o;
-      if (d == 0) {
-        float* const at = a.partial + (int64_t)a.sequences * a.heads * a.parts * a.dim + row * 2;
-        at[0] = all_top;
-        at[1] = total;
-      }
-    } else {
-      const float inverse = total == 0.0f ? 0.0f : a.value_scale / total;
+    if (g == 0) {
+      float* const stats = a.partial + (int64_t)a.sequences * a.heads * a.parts * a.dim + at * 2;
+      stats[0] = top;
+      stats[1] = sum;
+    }
+  } else {
+    const float inverse = sum == 0.0f ? 0.0f : a.value_scale / sum;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) T::Codec::store1(a.out, head * a.dim + d + j, total == 0.0f ? 0.0f : o[j] * inverse);
-      if (d == 0 && a.lse != nullptr) {
-        a.lse[head] = total == 0.0f ? -__builtin_inff() : (all_top + __builtin_log2f(total)) * kLn2;
+    for (int f = 0; f < kOut; ++f) {
+      if (16 * f < a.dim) {
+        const f32x4 o = sum == 0.0f ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : out[f] * inverse;
+        store4<typename T::Codec>(o, a.out + (head * a.dim + 16 * f + 4 * g) * T::kBytes);
       }
+    }
+    if (g == 0 && a.lse != nullptr) {
+      a.lse[head] = sum == 0.0f ? -__builtin_inff() : (top + __builtin_log2f(sum)) * kLn2;
     }
   }
 }
@@ -435,11 +532,11 @@ int parts_of(int64_t sequences, int64_t units, int64_t positions) {
 template <class T, class S>
 int32_t run_dim(const AttentionArgs& a, int64_t blocks, hipStream_t st) {
   if (a.dim <= 64) {
-    paged_attention<T, S, 64><<<(unsigned)blocks, kWaves * 64, 0, st>>>(a);
+    paged_attention<T, S, 64><<<(unsigned)blocks, 64, 0, st>>>(a);
   } else if (a.dim <= 128) {
-    paged_attention<T, S, 128><<<(unsigned)blocks, kWaves * 64, 0, st>>>(a);
+    paged_attention<T, S, 128><<<(unsigned)blocks, 64, 0, st>>>(a);
   } else {
-    paged_attention<T, S, 256><<<(unsigned)blocks, kWaves * 64, 0, st>>>(a);
+    paged_attention<T, S, 256><<<(unsigned)blocks, 64, 0, st>>>(a);
   }
   int32_t status = launch_status();
   if (status == 0 && a.parts > 1) {
@@ -486,7 +583,7 @@ extern "C" int32_t launch_paged_attention_fwd(const void* q, const void* key_cac
   if (cache_dtype != dtype && cache_dtype != kF8E4M3 && cache_dtype != kF8E5M2) return (int32_t)hipErrorInvalidValue;
   if (sequences <= 0 || n_q_heads <= 0) return (int32_t)hipSuccess;
   if (!attention_sizes_ok(sequences, n_q_heads, n_kv_heads, head_dim, page_size, table_width) || pages < 0 ||
-      pages > INT64_MAX / page_size / n_kv_heads / head_dim / 4) {
+      pages > INT32_MAX / page_size) {
     return (int32_t)hipErrorInvalidValue;
   }
   AttentionArgs a = {};

@@ -296,7 +296,8 @@ int32_t launch_rope_to_cache_fwd(const void* q, const void* k, const void* v, vo
  * h / (n_q_heads / n_kv_heads). q: one token a sequence. Caches [pages, page_size,
  * n_kv_heads, head_dim] of dtype or FP8; position t of sequence b is at place t %
  * page_size of page page_table[b][t / page_size]. Seen are the positions below
- * lengths[b] (at most table_width * page_size, which is at most 2^30) and, with window >
+ * lengths[b] (at most table_width * page_size, which is at most 2^30; the caches hold
+ * fewer than 2^31 positions) and, with window >
  * 0, the last `window` of them; positions on a page outside [0, pages) are left out.
  * Where none is left, out is zeros and lse -infinity. lse [sequences, n_q_heads]: log of
  * the sum of the exponentials, or NULL. head_dim: a multiple of 16, at most 256.
