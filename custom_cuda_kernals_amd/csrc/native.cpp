@@ -1077,9 +1077,8 @@ PYBIND11_MODULE(_native, m) {
   m.def("paged_attention_fwd", &paged_attention_fwd, py::arg("q"), py::arg("key_cache"), py::arg("value_cache"),
         py::arg("page_table"), py::arg("lengths"), py::arg("out"), py::arg("lse"), py::arg("workspace"),
         py::arg("scale"), py::arg("window"), py::arg("key_scale"), py::arg("value_scale"));
-  m.def("paged_attention_workspace", &cck_paged_attention_workspace, py::arg("sequences"), py::arg("heads"),
-        py::arg("kv_heads"), py::arg("head_dim"), py::arg("page_size"), py::arg("table_width"),
-        "Bytes of the workspace that paged_attention_fwd takes.");
+  m.def("paged_attention_workspace", &paged_attention_workspace, py::arg("q"), py::arg("key_cache"),
+        py::arg("page_table"), "Bytes of the workspace that paged_attention_fwd takes for these.");
   // The Python API in one call each (native_calls.hpp).
   if (PyModule_AddFunctions(m.ptr(), calls::kMethods) != 0) throw py::error_already_set();
 }

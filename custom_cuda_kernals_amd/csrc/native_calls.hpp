@@ -778,7 +778,7 @@ inline PyObject* paged_attention(PyObject*, PyArgs a, Py_ssize_t n) {
     Py_RETURN_NONE;
   }
   const int64_t stats[2] = {qh.tokens, qh.heads};
-  const int64_t bytes = cck_paged_attention_workspace(qh.tokens, qh.heads, kv, qh.dim, page, width);
+  const int64_t bytes = cck_paged_attention_workspace(qh.tokens, qh.heads, kv, qh.dim, page, width, tag);
   const int64_t room[1] = {bytes / 4}, none[1] = {0};
   const Launch launch(q.device().index());
   at::Tensor out[3];

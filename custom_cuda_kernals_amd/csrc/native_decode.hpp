@@ -226,6 +226,15 @@ const char* attention_limits(int64_t sequences, int64_t heads, int64_t kv_heads,
   return nullptr;
 }
 
+// 0 for what paged_attention_fwd refuses.
+int64_t paged_attention_workspace(py::handle q, py::handle key_cache, py::handle page_table) {
+  const HeadsView qv = validate_heads("q", q);
+  const RawView kv = validate_and_extract("key_cache", key_cache), tv = validate_and_extract("page_table", page_table);
+  const auto tag = tag_from_dtype_str(kv.dtype_str);
+  if (qv.v.shape.size() != 3 || kv.shape.size() != 4 || tv.shape.size() != 2 || !tag) return 0;
+  return cck_paged_attention_workspace(qv.tokens, qv.heads, kv.shape[2], qv.dim, kv.shape[1], tv.shape[1], *tag);
+}
+
 void paged_attention_fwd(py::handle q, py::handle key_cache, py::handle value_cache, py::handle page_table,
                          py::handle lengths, py::handle out, py::handle lse, py::handle workspace, double scale,
                          int64_t window, double key_scale, double value_scale) {
@@ -265,7 +274,7 @@ void paged_attention_fwd(py::handle q, py::handle key_cache, py::handle value_ca
     if (ev->shape != std::vector<int64_t>{qv.tokens, qv.heads}) shape_mismatch("lse must be [sequences, heads]");
   }
   const int64_t bytes =
-      cck_paged_attention_workspace(qv.tokens, qv.heads, kv_heads, qv.dim, kc.shape[1], tv.shape[1]);
+      cck_paged_attention_workspace(qv.tokens, qv.heads, kv_heads, qv.dim, kc.shape[1], tv.shape[1], kc.dtype);
   if (!workspace.is_none()) {
     wv = validate_tensor("workspace", workspace);
     require_f32("workspace", *wv);

@@ -15,9 +15,10 @@
 // one product to the other inside the lane. 16-bit P is split in two parts, high and low:
 // rounded once, it would add an error as large as that of the output's own rounding.
 //
-// Bound by HBM: reading keys and values once. A sequence is cut into parts for as many
-// waves as fill the card; a workgroup is one wave with one part of one key-value head, and
-// the parts' sums meet in a second launch. Keys and values go straight from memory to LDS,
+// Bound by HBM: reading keys and values once. The sequences are cut into parts of one
+// length, as many as fill the card; a workgroup is one wave with one part of one key-value
+// head, and the parts' sums meet in a second launch. The lengths are on the GPU, so each
+// workgroup finds its part itself, from the sum of all lengths. Keys and values go straight from memory to LDS,
 // whole rows at a time, into a ring of two steps: a step is on its way while the one
 // before is worked on, without registers or other waves to wait for.
 #include "tile_product.hpp"
@@ -38,9 +39,12 @@ struct AttentionArgs {
   const char *q, *keys, *values;
   const int64_t *table, *lengths;
   char* out;
-  float *lse, *partial;  // partial: [sequence][key-value head][part][G][dim], then [..][G][2]
+  // partial: [parts][heads][dim], then [parts][heads][2], the maximum and the sum, and then of each sequence
+  // its first part and how many it has.
+  float *lse, *partial;
   int64_t q_token, q_head, pages;
-  int sequences, heads, kv_heads, dim, page, table_width, window, parts, head_tiles;
+  int sequences, heads, kv_heads, dim, page, table_width, window, head_tiles;
+  int parts;  // of all sequences together, at most; 0: each sequence is one
   uint32_t page_magic;
   int page_shift;
   float score_scale, value_scale;  // score_scale: with log2(e)
@@ -111,22 +115,108 @@ struct FromCodes {
   }
 };
 
-// Positions [lo, hi) of a sequence that are seen, and of one of its parts; count: its parts.
-struct Span {
-  int lo, hi, begin, end, count;
-  __device__ Span(const AttentionArgs& a, int sequence, int part) {
+// The positions of a sequence that are seen: [lo, lo + seen).
+struct Seen {
+  int lo, seen;
+  __device__ Seen(const AttentionArgs& a, int sequence) {
     const int64_t most = (int64_t)a.table_width * a.page;
     int64_t n = a.lengths[sequence];
     n = n < 0 ? 0 : n > most ? most : n;
-    hi = __builtin_amdgcn_readfirstlane((int)n);
-    lo = a.window > 0 && hi > a.window ? hi - a.window : 0;
-    const int seen = hi - lo;
-    int each = (seen + a.parts - 1) / a.parts;
-    each = (each + kMinPart - 1) / kMinPart * kMinPart;
+    lo = a.window > 0 && n > a.window ? (int)n - a.window : 0;
+    seen = (int)n - lo;
+  }
+};
+
+__device__ inline float* stats_of(const AttentionArgs& a) { return a.partial + (int64_t)a.parts * a.heads * a.dim; }
+__device__ inline int* notes_of(const AttentionArgs& a) {
+  return reinterpret_cast<int*>(stats_of(a) + (int64_t)a.parts * a.heads * 2);
+}
+
+// How the sequences are cut: into parts of `each` positions, numbered through all of them.
+// A lane has a run of sequences, and knows how many parts come before them. Every lane of
+// the wave calls.
+struct Cut {
+  int each, run, mine, before, all;  // sequences of a run; parts of the lane's, before them, and of all
+  __device__ Cut(const AttentionArgs& a) : run((a.sequences + 63) / 64) {
+    const int first = (int)(threadIdx.x & 63) * run;
+    double total = 0.0;  // exact: below 2^41
+    for (int i = 0; i < run; ++i) {
+      if (first + i < a.sequences) total += (double)Seen(a, first + i).seen;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+    // Each sequence has a last part that may be short, so that there are no more than a.parts in all.
+    const int wanted = (int)__builtin_ceil(total / (double)(a.parts - a.sequences));
+    each = __builtin_amdgcn_readfirstlane((wanted + kMinPart - 1) / kMinPart * kMinPart);
     each = each < kMinPart ? kMinPart : each;
-    count = (seen + each - 1) / each;
-    begin = lo + part * each;
-    end = begin + each < hi ? begin + each : hi;
+    mine = 0;
+    for (int i = 0; i < run; ++i) mine += parts_of(a, first + i);
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int v = __shfl_up(sum, d);
+      if ((int)(threadIdx.x & 63) >= d) sum += v;
+    }
+    before = sum - mine;
+    all = __builtin_amdgcn_readlane(sum, 63);
+  }
+  __device__ int parts_of(const AttentionArgs& a, int sequence) const {
+    return sequence < a.sequences ? (Seen(a, sequence).seen + each - 1) / each : 0;
+  }
+  // First part and number of parts of each sequence, for the launch that joins them.
+  __device__ void note(const AttentionArgs& a) const {
+    int* const notes = notes_of(a);
+    int at = before;
+    for (int i = 0; i < run; ++i) {
+      const int s = (int)(threadIdx.x & 63) * run + i, n = parts_of(a, s);
+      if (s < a.sequences) {
+        notes[2 * s] = at;
+        notes[2 * s + 1] = n;
+      }
+      at += n;
+    }
+  }
+};
+
+// A workgroup's work: positions [begin, end) of a sequence that has `count` parts, and which
+// heads. All heads of a part go to one XCD, one after another. In turn they would go to the
+// XCDs in turn too, and an XCD then read the same few hundred bytes of each row of heads,
+// which are the same few channels of its L2.
+struct Part {
+  int index = 0, unit = 0, sequence = 0, begin = 0, end = 0, count = 1;
+  bool none = false;
+  __device__ Part(const AttentionArgs& a, int id) {
+    const int units = a.kv_heads * a.head_tiles;
+    int part = 0, each = INT32_MAX;
+    if (a.parts == 0) {
+      id = xcd_contiguous(id, a.sequences * units);
+      sequence = index = id / units;
+      unit = id - index * units;
+    } else {
+      const Cut cut(a);
+      each = cut.each;
+      if (id == 0) cut.note(a);
+      none = id >= cut.all * units;
+      if (none) return;
+      id = xcd_contiguous(id, cut.all * units);
+      index = id / units;
+      unit = id - index * units;
+      const uint64_t owner = __ballot(index >= cut.before && index < cut.before + cut.mine);
+      int at = cut.before, found = 0, in = 0;
+      for (int i = 0; i < cut.run; ++i) {
+        const int s = (int)(threadIdx.x & 63) * cut.run + i, n = cut.parts_of(a, s);
+        if (index >= at && index < at + n) found = s, in = index - at;
+        at += n;
+      }
+      const int lane = __builtin_ctzll(owner);
+      sequence = __builtin_amdgcn_readlane(found, lane);
+      part = __builtin_amdgcn_readlane(in, lane);
+    }
+    const Seen s(a, sequence);
+    const int seen = __builtin_amdgcn_readfirstlane(s.seen), lo = __builtin_amdgcn_readfirstlane(s.lo);
+    if (a.parts > 0) count = (seen + each - 1) / each;
+    begin = lo + part * (a.parts > 0 ? each : 0);
+    end = seen - part * (a.parts > 0 ? each : 0) <= each ? lo + seen : begin + each;
   }
 };
 
@@ -170,9 +260,10 @@ __device__ inline void store4(const f32x4& v, char* p) {
   }
 }
 
-// 16 bytes per lane from p to LDS at the named place + 16 x lane (see lds_place).
+// 16 bytes per lane from p to LDS at the named place + 16 x lane (see lds_place), as data that is
+// read once: 207 us in place of 236 for the 64 ragged sequences below.
 __device__ inline void load_to_place_from(const char* p) {
-  asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(p) : "memory");
+  asm volatile("global_load_lds_dwordx4 %0, off nt" ::"v"(p) : "memory");
 }
 
 // FP8 values of element 16 f + col and eight positions, 4 g .. 4 g + 3 and 16 on: lanes 2 j
@@ -194,15 +285,11 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[kDepth * Sh::kSlot];
   __shared__ int found[kFound];
 
-  const int units = a.kv_heads * a.head_tiles;
-  int id = blockIdx.x;
-  const int unit = id % units;
-  id /= units;
-  const int sequence = id % a.sequences, part = id / a.sequences;
+  const Part span(a, (int)blockIdx.x);
+  if (span.none) return;
+  const int sequence = span.sequence, index = span.index, unit = span.unit;
   const int kv = unit / a.head_tiles, group = a.heads / a.kv_heads;
   const int head0 = unit % a.head_tiles * kHeads, heads = group - head0 < kHeads ? group - head0 : kHeads;
-  const Span span(a, sequence, part);
-  if (part >= span.count && part > 0) return;
 
   const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
   const int row_bytes = a.dim * S::kBytes;
@@ -445,15 +532,16 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
   sum += __shfl_xor(sum, 32);
 
   if (col >= heads) return;
-  const int64_t head = (int64_t)sequence * a.heads + kv * group + head0 + col;
-  if (a.parts > 1) {
-    const int64_t at = head * a.parts + part;
+  const int in_sequence = kv * group + head0 + col;
+  const int64_t head = (int64_t)sequence * a.heads + in_sequence;
+  if (span.count > 1) {
+    const int64_t at = (int64_t)index * a.heads + in_sequence;
 #pragma unroll
     for (int f = 0; f < kOut; ++f) {
       if (16 * f < a.dim) *reinterpret_cast<f32x4*>(a.partial + at * a.dim + 16 * f + 4 * g) = out[f];
     }
     if (g == 0) {
-      float* const stats = a.partial + (int64_t)a.sequences * a.heads * a.parts * a.dim + at * 2;
+      float* const stats = stats_of(a) + at * 2;
       stats[0] = top;
       stats[1] = sum;
     }
@@ -472,61 +560,92 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
   }
 }
 
-// The parts' sums, a head a workgroup.
-template <class C>
-__global__ __launch_bounds__(256) void join_parts(AttentionArgs a) {
-  __shared__ float weights[256];
-  __shared__ f32x4 sums[256];
-  const int64_t head = blockIdx.x;
-  const Span span(a, (int)(head / a.heads), 0);
-  const int count = span.count, tid = threadIdx.x;
-  const float* const stats = a.partial + (int64_t)a.sequences * a.heads * a.parts * a.dim + head * a.parts * 2;
-  float top = -__builtin_inff();
-  for (int i = tid & 63; i < count; i += 64) top = __builtin_fmaxf(top, stats[2 * i]);
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) top = __builtin_fmaxf(top, __shfl_xor(top, d));
-  const float base = top == -__builtin_inff() ? 0.0f : top;
-  float total = 0.0f;
-  for (int i = tid & 63; i < count; i += 64) {
-    const float w = __builtin_amdgcn_exp2f(stats[2 * i] - base);
-    total += w * stats[2 * i + 1];
-    if (tid < 64 && i < 256) weights[i] = w;
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
-  __syncthreads();
-  // Threads of one quad of elements take every `lanes`-th part.
-  const int quads = a.dim / 4, lanes = 256 / quads, quad = tid % quads, of = tid / quads;
+constexpr int kMaxParts = 1024;  // of all sequences, or twice as many as there are of them
+constexpr int64_t kMaxPositions = int64_t(1) << 30;  // of a sequence: a step past the last is still an int
+constexpr int kMaxCut = 2048;  // sequences: beyond it each is one part, so that nobody reads so many lengths
+
+// The sums of a sequence's parts, a head a workgroup. A thread has four elements of every
+// `lanes`-th part, and takes kAhead parts at a time.
+template <class C, int THREADS>
+__global__ __launch_bounds__(THREADS) void join_parts(AttentionArgs a) {
+  __shared__ f32x4 sums[THREADS];
+  __shared__ f32x2 tops[THREADS];
+  constexpr int kAhead = THREADS == 64 ? 4 : 8;
+  const int sequence = (int)(blockIdx.x / a.heads), head = (int)(blockIdx.x - sequence * a.heads);
+  const int* const notes = notes_of(a) + 2 * sequence;
+  const int first = notes[0], count = notes[1], tid = threadIdx.x;
+  if (count == 1) return;  // its wave stored the result
+  const int quads = a.dim / 4, lanes = THREADS / quads, quad = tid % quads, of = tid / quads;
+  const float* const from = a.partial + ((int64_t)first * a.heads + head) * a.dim + quad * 4;
+  const f32x2* const stats = reinterpret_cast<const f32x2*>(stats_of(a)) + (int64_t)first * a.heads + head;
+  const int64_t stride = (int64_t)a.heads * a.dim;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  float top = -__builtin_inff(), total = 0.0f;
   if (of < lanes) {
-    const float* from = a.partial + head * a.parts * a.dim + quad * 4;
-    for (int i = of; i < count; i += lanes) o += weights[i] * *reinterpret_cast<const f32x4*>(from + (int64_t)i * a.dim);
+    for (int p0 = of; p0 < count; p0 += kAhead * lanes) {
+      f32x4 part[kAhead];
+      f32x2 stat[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int p = p0 + i * lanes, at = p < count ? p : p0;
+        part[i] = *reinterpret_cast<const f32x4*>(from + at * stride);
+        stat[i] = stats[(int64_t)at * a.heads];
+        if (p >= count) stat[i] = (f32x2){-__builtin_inff(), 0.0f};
+      }
+      const float before = top;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) top = __builtin_fmaxf(top, stat[i][0]);
+      const float base = top == -__builtin_inff() ? 0.0f : top, keep = __builtin_amdgcn_exp2f(before - base);
+      o *= keep;
+      total *= keep;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const float w = __builtin_amdgcn_exp2f(stat[i][0] - base);
+        if (p0 + i * lanes < count) o += w * part[i];
+        total += w * stat[i][1];
+      }
+    }
   }
   sums[tid] = o;
+  tops[tid] = (f32x2){top, total};
   __syncthreads();
-  if (tid < quads) {
-    for (int i = 1; i < lanes; ++i) o += sums[i * quads + tid];
-    const float inverse = total == 0.0f ? 0.0f : a.value_scale / total;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) C::store1(a.out, head * a.dim + tid * 4 + j, total == 0.0f ? 0.0f : o[j] * inverse);
-    if (tid == 0 && a.lse != nullptr) {
-      a.lse[head] = total == 0.0f ? -__builtin_inff() : (top + __builtin_log2f(total)) * kLn2;
-    }
+  if (tid >= quads) return;
+  float all_top = top;
+  for (int i = 1; i < lanes; ++i) all_top = __builtin_fmaxf(all_top, tops[i * quads + tid][0]);
+  const float base = all_top == -__builtin_inff() ? 0.0f : all_top;
+  o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  total = 0.0f;
+  for (int i = 0; i < lanes; ++i) {
+    const float w = __builtin_amdgcn_exp2f(tops[i * quads + tid][0] - base);
+    o += w * sums[i * quads + tid];
+    total += w * tops[i * quads + tid][1];
+  }
+  const float inverse = total == 0.0f ? 0.0f : a.value_scale / total;
+  o = total == 0.0f ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : o * inverse;
+  store4<C>(o, a.out + ((int64_t)blockIdx.x * a.dim + tid * 4) * C::kBytes);
+  if (tid == 0 && a.lse != nullptr) {
+    a.lse[blockIdx.x] = total == 0.0f ? -__builtin_inff() : (all_top + __builtin_log2f(total)) * kLn2;
   }
 }
 
-constexpr int kMaxParts = 256;  // join_parts holds a weight for each
-constexpr int64_t kMaxPositions = int64_t(1) << 30;  // of a sequence: a step past the last is still an int
+int64_t bytes_of(int32_t dtype) { return dtype == kF32 ? 4 : dtype == kF16 || dtype == kBF16 ? 2 : 1; }
 
 int head_tiles_of(int64_t heads, int64_t kv_heads) { return (int)((heads / kv_heads + kHeads - 1) / kHeads); }
 
-// Parts of a sequence: as many as make 2048 workgroups, of kMinPart positions at least.
-int parts_of(int64_t sequences, int64_t units, int64_t positions) {
-  const int64_t groups = sequences * units, wanted = (2048 + groups - 1) / groups;
-  const int64_t most = (positions + kMinPart - 1) / kMinPart;
-  int64_t parts = wanted < most ? wanted : most;
-  parts = parts < kMaxParts ? parts : kMaxParts;
-  return (int)(parts < 1 ? 1 : parts);
+// Parts of all sequences together, or 0 where each is one: as many as fill the LDS of the
+// 256 CUs, and eight times the sequences, for lengths that differ.
+int parts_of(int64_t sequences, int64_t units, int64_t positions, int64_t dim, int64_t cache_bytes) {
+  if (positions <= kMinPart || sequences > kMaxCut) return 0;
+  const int64_t padded = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+  const int64_t step = (cache_bytes == 4 ? 16 : 32) * padded * cache_bytes * 2;
+  const int64_t of_cu = 160 * 1024 / (kDepth * step + kFound * 4);
+  const int64_t slots = 256 * (of_cu < 8 ? of_cu : 8);
+  int64_t parts = (slots + units - 1) / units;
+  parts = parts > 8 * sequences ? parts : 8 * sequences;
+  const int64_t limit = 2 * sequences > kMaxParts ? 2 * sequences : kMaxParts;
+  parts = parts < limit ? parts : limit;
+  const int64_t most = sequences * ((positions + kMinPart - 1) / kMinPart) + sequences;  // of the shortest parts
+  return (int)(parts < most ? parts : most);
 }
 
 template <class T, class S>
@@ -539,8 +658,14 @@ int32_t run_dim(const AttentionArgs& a, int64_t blocks, hipStream_t st) {
     paged_attention<T, S, 256><<<(unsigned)blocks, 64, 0, st>>>(a);
   }
   int32_t status = launch_status();
-  if (status == 0 && a.parts > 1) {
-    join_parts<typename T::Codec><<<(unsigned)(a.sequences * a.heads), 256, 0, st>>>(a);
+  if (status == 0 && a.parts > 0) {
+    // Few parts a sequence on average: a wave for each head (64 sequences of up to 8 parts: 5 us less).
+    const unsigned grid = (unsigned)(a.sequences * a.heads);
+    if (a.parts <= 16 * (int64_t)a.sequences) {
+      join_parts<typename T::Codec, 64><<<grid, 64, 0, st>>>(a);
+    } else {
+      join_parts<typename T::Codec, 512><<<grid, 512, 0, st>>>(a);
+    }
     status = launch_status();
   }
   return status;
@@ -566,10 +691,12 @@ bool attention_sizes_ok(int64_t sequences, int64_t heads, int64_t kv_heads, int6
 using namespace cck;
 
 extern "C" int64_t cck_paged_attention_workspace(int64_t sequences, int64_t n_q_heads, int64_t n_kv_heads,
-                                                 int64_t head_dim, int64_t page_size, int64_t table_width) {
+                                                 int64_t head_dim, int64_t page_size, int64_t table_width,
+                                                 int32_t cache_dtype) {
   if (sequences <= 0 || !attention_sizes_ok(sequences, n_q_heads, n_kv_heads, head_dim, page_size, table_width)) return 0;
-  const int parts = parts_of(sequences, n_kv_heads * head_tiles_of(n_q_heads, n_kv_heads), page_size * table_width);
-  return parts == 1 ? 0 : sequences * n_q_heads * parts * (head_dim + 2) * 4;
+  const int64_t units = n_kv_heads * head_tiles_of(n_q_heads, n_kv_heads);
+  const int64_t parts = parts_of(sequences, units, page_size * table_width, head_dim, bytes_of(cache_dtype));
+  return parts == 0 ? 0 : parts * n_q_heads * (head_dim + 2) * 4 + sequences * 8;
 }
 
 extern "C" int32_t launch_paged_attention_fwd(const void* q, const void* key_cache, const void* value_cache,
@@ -606,8 +733,9 @@ extern "C" int32_t launch_paged_attention_fwd(const void* q, const void* key_cac
   a.table_width = pages > 0 ? (int)table_width : 0;  // no page: no position
   a.window = window > 0 && window < INT32_MAX ? (int)window : 0;
   a.head_tiles = head_tiles_of(n_q_heads, n_kv_heads);
-  a.parts = parts_of(sequences, n_kv_heads * a.head_tiles, page_size * table_width);
-  if (a.parts > 1 && (workspace == nullptr || !host_aligned(workspace, 16))) return (int32_t)hipErrorInvalidValue;
+  const int64_t units = n_kv_heads * a.head_tiles;
+  a.parts = parts_of(sequences, units, page_size * table_width, head_dim, bytes_of(cache_dtype));
+  if (a.parts > 0 && (workspace == nullptr || !host_aligned(workspace, 16))) return (int32_t)hipErrorInvalidValue;
   // t / page for t < 2^31: t * magic >> shift, magic = floor(2^(31 + bits) / page) + 1 with
   // 2^bits >= page. What magic is too large by, at most 1, adds less than 2^-bits <= 1 / page.
   int bits = 0;
@@ -616,7 +744,7 @@ extern "C" int32_t launch_paged_attention_fwd(const void* q, const void* key_cac
   a.page_magic = (uint32_t)(((unsigned __int128)1 << (31 + bits)) / (uint64_t)page_size + 1);
   a.score_scale = scale * key_scale * kLog2e;
   a.value_scale = value_scale;
-  const int64_t blocks = sequences * n_kv_heads * a.head_tiles * a.parts;
+  const int64_t blocks = (a.parts > 0 ? a.parts : sequences) * units;
   if (blocks > (int64_t(1) << 24) - 1) return (int32_t)hipErrorInvalidValue;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {

@@ -67,11 +67,8 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
         return out
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
-    workspace = None
-    if q.dim() == 3 and key_cache.dim() == 4 and page_table.dim() == 2:
-        bytes_ = native.paged_attention_workspace(q.shape[0], q.shape[1], key_cache.shape[2], q.shape[2],
-                                                  key_cache.shape[1], page_table.shape[1])
-        workspace = torch.empty(bytes_ // 4, dtype=torch.float32, device=q.device)
+    bytes_ = native.paged_attention_workspace(q, key_cache, page_table)
+    workspace = torch.empty(bytes_ // 4, dtype=torch.float32, device=q.device)
     native.paged_attention_fwd(q, key_cache, value_cache, page_table, lengths, out, lse, workspace, scale, int(window),
                                float(key_scale), float(value_scale))
     return (out, lse) if return_lse else out

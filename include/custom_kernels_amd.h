@@ -311,7 +311,7 @@ int32_t launch_paged_attention_fwd(const void* q, const void* key_cache, const v
                                    float key_scale, float value_scale, int32_t dtype, int32_t cache_dtype,
                                    void* stream);
 int64_t cck_paged_attention_workspace(int64_t sequences, int64_t n_q_heads, int64_t n_kv_heads, int64_t head_dim,
-                                      int64_t page_size, int64_t table_width);
+                                      int64_t page_size, int64_t table_width, int32_t cache_dtype);
 
 /* ---- FP8 with a scale for each block of 128 (no reference counterpart) ---- */
 

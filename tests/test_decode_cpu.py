@@ -316,7 +316,7 @@ def test_launchers_refuse_and_take_nothing():
     assert cache(tokens=0) == 0
     assert cache(key_scale=0.0) == 1 and cache(key_scale=math.inf) == 1 and cache(cache_dtype=1) == 1 and cache(half=40) == 1
 
-    def attention(sequences=1, heads=8, kv=2, dim=64, page=16, width=4, dtype=2, cache_dtype=2, workspace=None):
+    def attention(sequences=1, heads=8, kv=2, dim=64, page=16, width=2, dtype=2, cache_dtype=2, workspace=None):
         return lib.launch_paged_attention_fwd(p, p, p, p, p, p, None, workspace, 512, 64, sequences, heads, kv, dim, 9, page,
                                               width, 0, 1.0, 1.0, 1.0, dtype, cache_dtype, None)
 
@@ -326,8 +326,8 @@ def test_launchers_refuse_and_take_nothing():
                 {"sequences": 1 << 23}):
         assert attention(**bad) == 1, bad
     room = lib.cck_paged_attention_workspace
-    room.restype, room.argtypes = ctypes.c_int64, [ctypes.c_int64] * 6
-    assert room(1, 8, 2, 64, 16, 4) == 0 and room(1, 8, 2, 64, 16, 400) > 0 and room(1, 7, 2, 64, 16, 400) == 0
+    room.restype, room.argtypes = ctypes.c_int64, [ctypes.c_int64] * 6 + [ctypes.c_int32]
+    assert room(1, 8, 2, 64, 16, 2, 2) == 0 and room(1, 8, 2, 64, 16, 400, 3) > 0 and room(1, 7, 2, 64, 16, 400, 2) == 0
 
     def linear(rows=1, experts=1, n=16, k=128, block_rows=1, fx=3, fw=3, dtype=2):
         return lib.launch_fp8_block_linear_fwd(p, p, p, p, None, p, rows, experts, n, k, block_rows, fx, fw, dtype, None)
