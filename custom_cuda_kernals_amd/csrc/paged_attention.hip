@@ -29,7 +29,7 @@ namespace {
 constexpr int kHeads = 16;    // query heads of a workgroup, at most
 constexpr int kMinPart = 32;  // positions of a part, at least: a step
 constexpr int kFound = 512;   // positions whose slots are looked up at a time
-constexpr int kDepth = 2;     // steps in LDS
+constexpr int kRing = 32768;  // bytes of LDS for the steps of a wave: more only if two steps need it
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Sums are scaled to a new maximum only where it is this much (a power of two) above the
 // one that they have.
@@ -233,6 +233,7 @@ struct Shape {
   static constexpr int kRows = 64 / kChunks;             // that one load instruction brings
   static constexpr int kLoads = kStep / kRows;           // of a step, of keys or of values
   static constexpr int kKeys = kStep * kRow, kSlot = 2 * kKeys;
+  static constexpr int kDepth = kSlot >= kRing / 2 ? 2 : kRing / kSlot;  // steps in LDS
   static_assert(kChunks % 4 == 0 && kRows >= 1 && kRows <= 16 && 2 * kLoads < 64);
   // A lane reads a chunk of one of 16 neighbouring rows.
   __device__ static int key_place(int r) { return kChunks >= 8 ? r & 7 : (r ^ (r >> 2)) & 3; }
@@ -282,6 +283,7 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
   using Sh = Shape<T, S, DIM>;
   constexpr int kTiles = Sh::kTiles, kStep = Sh::kStep, kOfLane = Sh::kOfLane, kFrags = S::kFragments;
   constexpr int kRow = Sh::kRow, kAll = 2 * Sh::kLoads;
+  constexpr int kDepth = Sh::kDepth;
   __shared__ __attribute__((aligned(1024))) char lds[kDepth * Sh::kSlot];
   __shared__ int found[kFound];
 
@@ -515,7 +517,7 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
     for (int d = 0; d < kDepth; ++d) {
       const int now = first + d * kStep;
       if (now < end) {
-        if (now + kStep < end) {
+        if (now + (kDepth - 1) * kStep < end) {
           loads_landed<(kDepth - 1) * kAll>();
         } else {
           loads_landed();
@@ -637,9 +639,8 @@ int head_tiles_of(int64_t heads, int64_t kv_heads) { return (int)((heads / kv_he
 int parts_of(int64_t sequences, int64_t units, int64_t positions, int64_t dim, int64_t cache_bytes) {
   if (positions <= kMinPart || sequences > kMaxCut) return 0;
   const int64_t padded = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-  const int64_t step = (cache_bytes == 4 ? 16 : 32) * padded * cache_bytes * 2;
-  const int64_t of_cu = 160 * 1024 / (kDepth * step + kFound * 4);
-  const int64_t slots = 256 * (of_cu < 8 ? of_cu : 8);
+  const int64_t two = (cache_bytes == 4 ? 16 : 32) * padded * cache_bytes * 2 * 2;
+  const int64_t slots = 256 * (160 * 1024 / ((two > kRing ? two : kRing) + kFound * 4));
   int64_t parts = (slots + units - 1) / units;
   parts = parts > 8 * sequences ? parts : 8 * sequences;
   const int64_t limit = 2 * sequences > kMaxParts ? 2 * sequences : kMaxParts;
