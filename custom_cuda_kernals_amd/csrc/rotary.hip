@@ -8,9 +8,9 @@
 // factor s the rotation is s times an orthogonal map. launch_rope_at_fwd writes q and k;
 // launch_rope_to_cache_fwd writes q, and k and v to slots of a paged cache.
 //
-// Bound by HBM, q and k once each way. The angles are not read but made: a workgroup has a
-// few tokens, and each of its threads the sine and cosine of one (token, pair), into LDS,
-// while its first vectors are on their way. The angle is formed in float64, where whole
+// Bound by HBM, q and k once each way. The angles are not read but made: each thread of a
+// workgroup the sine and cosine of a (token, pair), into LDS, while its vectors are on
+// their way. The angle is formed in float64, where whole
 // turns come off exactly: position 10^6 keeps the last bits that float32 angles lose from
 // some hundred positions on.
 #include "launch.hpp"
@@ -18,9 +18,12 @@
 namespace cck {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kInFlight = 4;        // items of a thread whose loads are issued together
-constexpr int kMaxHalf = 1024;      // pairs of a head
+constexpr int kMaxThreads = 1024, kFewThreads = 128;
+constexpr int64_t kMaxGroups = int64_t(1) << 21;  // workgroups; beyond it they loop
+constexpr int kMaxHalf = 1024;                    // pairs of a head
+
+// The workgroup's LDS writes are there for all; loads that are on their way stay so, unlike at __syncthreads.
+__device__ inline void lds_written() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // sin and cos of position * frequency. In quarter turns the whole part picks the quadrant
 // and the rest, at most half a quarter turn, is exact in float64; its float32 rounding is
@@ -57,7 +60,7 @@ struct Args {
   const int64_t *positions, *slots;
   const double* frequencies;
   int64_t tokens, slot_count;
-  int dim, half, block_tokens, slices;
+  int dim, half;
   float factor, sine_sign, key_scale, key_inverse, value_scale, value_inverse;
 };
 
@@ -74,17 +77,12 @@ __host__ __device__ inline Pieces pieces_of(int dim, int half, bool copy) {
   return {half / kPairs, half % kPairs, rest / C::VEC, rest % C::VEC};
 }
 
-// Where results go: elements of C, or FP8 codes of a cache. NT: past the caches.
-template <class C, bool NT>
+// Where results go: elements of C, or FP8 codes of a cache.
+template <class C>
 struct Plain {
   static constexpr int kBytes = C::kBytes;
   __device__ static void vector(const float (&f)[C::VEC], char* p, float, float) {
-    const u32x4 w = C::pack(f);
-    if constexpr (NT) {
-      __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(p));
-    } else {
-      *reinterpret_cast<u32x4_any*>(p) = w;
-    }
+    *reinterpret_cast<u32x4_any*>(p) = C::pack(f);
   }
   __device__ static void one(float f, char* p, float, float) { C::store1(p, 0, f); }
 };
@@ -121,205 +119,183 @@ struct Codes {
 
 enum Kind { kNone, kTurnVector, kTurnPair, kCopyVector, kCopy };
 
-// One piece of one head of one token.
-template <class C, bool INTERLEAVED>
-struct Item {
-  static constexpr int kPairs = INTERLEAVED ? C::VEC / 2 : C::VEC;
-  int kind, target, first;  // target: 0 q, 1 k, 2 v; first: its first pair, or its first element if copied
-  uint32_t table;           // of its token
-  char* to;
-  u32x4 w[INTERLEAVED ? 1 : 2];
-  float a, b;
-};
-
 template <bool NT>
 __device__ inline u32x4 load16(const char* p) {
   if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
   return *reinterpret_cast<const u32x4_any*>(p);
 }
 
-// WHOLE: only vectors of pairs.
-template <class C, class KC, bool INTERLEAVED, bool CACHE, bool WHOLE, bool NT>
-__global__ __launch_bounds__(kThreads) void rope_at(Args a, int copy_q) {
-  using It = Item<C, INTERLEAVED>;
-  using QC = Plain<C, NT>;
-  extern __shared__ f32x2 table[];  // [block_tokens][half]: sine and cosine
+// A workgroup has TOKENS tokens, and a thread the same pieces of each: where they are is
+// found once, and the loads of all tokens go out together. blockIdx.y: which of a token's
+// pieces, where tokens are few.
+// WHOLE: only vectors of pairs, those of v being copied. NT: loads as of data read once, and stores that
+// go on from the caches at once, by 32-bit offsets in a token.
+template <class C, class KC, bool INTERLEAVED, bool CACHE, bool WHOLE, bool NT, int TOKENS>
+__global__ __launch_bounds__(kMaxThreads) void rope_at(Args a, int copy_q) {
+  constexpr int kPairs = INTERLEAVED ? C::VEC / 2 : C::VEC;
+  constexpr bool kCodes = CACHE && KC::kBytes != C::kBytes;
+  extern __shared__ f32x2 table[];  // [TOKENS][half]: sine and cosine
   const Pieces pq = pieces_of<C, INTERLEAVED>(a.dim, a.half, copy_q != 0);
   const Pieces pk = pieces_of<C, INTERLEAVED>(a.dim, a.half, CACHE || copy_q != 0);
-  // WHOLE: values in pieces as keys, which are not turned.
   const int value_vectors = a.dim / C::VEC, of_value = WHOLE ? pk.all() : value_vectors + a.dim % C::VEC;
   const int of_q = pq.all() * a.q.heads, of_qk = of_q + pk.all() * a.k.heads;
   const int of_token = of_qk + (CACHE ? of_value * a.v.heads : 0);
-  const int64_t groups = (a.tokens + a.block_tokens - 1) / a.block_tokens;
+  const int threads = (int)blockDim.x, stride = threads * (int)gridDim.y, begin = (int)blockIdx.y * threads;
+  const int64_t groups = (a.tokens + TOKENS - 1) / TOKENS;
+  // In registers: where one of several is taken, the compiler would put all arguments to scratch memory.
+  char *const q_to = a.q.to, *const k_to = a.k.to, *const v_to = a.v.to;
+  const int64_t cache_row = a.k.to_token * (kCodes ? KC::kBytes : C::kBytes);  // v's is as long
+  const float key_scale = a.key_scale, key_inverse = a.key_inverse, value_scale = a.value_scale,
+              value_inverse = a.value_inverse;
 
-  for (int64_t id = blockIdx.x; id < groups * a.slices; id += gridDim.x) {
-    const int64_t t0 = id / a.slices * a.block_tokens;
-    const int slice = (int)(id % a.slices);
-    const int count = a.tokens - t0 < a.block_tokens ? (int)(a.tokens - t0) : a.block_tokens;
-    const int total = count * of_token;
-    const int each = (total + a.slices - 1) / a.slices, begin = slice * each;
-    const int end = begin + each < total ? begin + each : total;
-
-    auto load = [&](int i, It& it) __attribute__((always_inline)) {
-      it.kind = kNone;
-      if (i >= end) return;
-      const int t = i / of_token;
-      int r = i - t * of_token, head, piece;
-      const int64_t token = t0 + t;
-      const Heads& h = r < of_q ? a.q : r < of_qk ? a.k : a.v;
-      it.target = r < of_q ? 0 : r < of_qk ? 1 : 2;
-      it.table = (uint32_t)(t * a.half);
-      Pieces p = it.target == 0 ? pq : pk;
-      if (it.target == 2) {
-        r -= of_qk;
-        if constexpr (!WHOLE) p = {0, 0, value_vectors, of_value - value_vectors};
-      } else if (it.target == 1) {
-        r -= of_q;
-      }
-      const int n = p.all();
-      head = r / n;
-      piece = r - head * n;
-      const char* from = h.from + (token * h.from_token + (int64_t)head * h.from_head) * C::kBytes;
-      const int bytes = CACHE && it.target > 0 ? KC::kBytes : C::kBytes;
-      int64_t row = token;
-      if (CACHE && it.target > 0) {
-        row = a.slots[token];
-        if (row < 0 || row >= a.slot_count) return;  // a token without a slot is not written
-      }
-      it.to = h.to + (row * h.to_token + (int64_t)head * h.to_head) * bytes;
-      if (piece < p.turn_vectors) {
-        it.kind = kTurnVector;
-        it.first = piece * It::kPairs;
-        const int e = INTERLEAVED ? 2 * it.first : it.first;
-        it.w[0] = load16<NT>(from + e * C::kBytes);
-        if constexpr (!INTERLEAVED) it.w[1] = load16<NT>(from + (e + a.half) * C::kBytes);
-        it.to += (int64_t)e * bytes;
-        return;
-      }
-      if constexpr (!WHOLE) {
-        piece -= p.turn_vectors;
-        if (piece < p.turn_pairs) {
-          it.kind = kTurnPair;
-          it.first = p.turn_vectors * It::kPairs + piece;
-          const int e = INTERLEAVED ? 2 * it.first : it.first;
-          it.a = C::load1(from, e);
-          it.b = C::load1(from, e + (INTERLEAVED ? 1 : a.half));
-          it.to += (int64_t)e * bytes;
-          return;
-        }
-        piece -= p.turn_pairs;
-        const int base = it.target == 2 ? 0 : 2 * a.half;
-        it.kind = piece < p.copy_vectors ? kCopyVector : kCopy;
-        const int e = base + (piece < p.copy_vectors ? piece * C::VEC
-                                                     : p.copy_vectors * C::VEC + piece - p.copy_vectors);
-        if (it.kind == kCopyVector) {
-          it.w[0] = load16<NT>(from + (int64_t)e * C::kBytes);
+  for (int64_t id = blockIdx.x; id < groups; id += gridDim.x) {
+    const int64_t t0 = id * TOKENS;
+    const int count = a.tokens - t0 < TOKENS ? (int)(a.tokens - t0) : TOKENS;
+    for (int i0 = begin; i0 < of_token; i0 += stride) {
+      // The thread's piece: of q (target 0), k or v, and where in a token.
+      const int i = i0 + (int)threadIdx.x;
+      int kind = kNone, target = 0, first = 0;  // first: its first pair
+      int64_t from = 0, to = 0;                 // bytes from the token's on
+      if (i < of_token) {
+        target = i < of_q ? 0 : i < of_qk ? 1 : 2;
+        Pieces p = target == 0 ? pq : pk;
+        if (!WHOLE && CACHE && target == 2) p = {0, 0, value_vectors, of_value - value_vectors};
+        const int r = i - (target == 0 ? 0 : target == 1 ? of_q : of_qk), head = r / p.all();
+        int piece = r - head * p.all(), e;
+        if (piece < p.turn_vectors) {
+          kind = kTurnVector;
+          first = piece * kPairs;
+          e = INTERLEAVED ? 2 * first : first;
+        } else if (piece -= p.turn_vectors; piece < p.turn_pairs) {
+          kind = kTurnPair;
+          first = p.turn_vectors * kPairs + piece;
+          e = INTERLEAVED ? 2 * first : first;
         } else {
-          it.a = C::load1(from, e);
+          piece -= p.turn_pairs;
+          kind = piece < p.copy_vectors ? kCopyVector : kCopy;
+          e = (CACHE && target == 2 ? 0 : 2 * a.half) +
+              (piece < p.copy_vectors ? piece * C::VEC : p.copy_vectors * C::VEC + piece - p.copy_vectors);
         }
-        it.to += (int64_t)e * bytes;
+        const int64_t from_head = target == 0 ? a.q.from_head : target == 1 ? a.k.from_head : a.v.from_head;
+        const int64_t to_head = target == 0 ? a.q.to_head : target == 1 ? a.k.to_head : a.v.to_head;
+        from = (head * from_head + e) * C::kBytes;
+        to = (head * to_head + e) * (kCodes && target > 0 ? KC::kBytes : C::kBytes);
       }
-    };
-
-    auto turn = [&](float& x, float& y, const f32x2& sc) {
-      const float u = __builtin_fmaf(x, sc[1], -(y * sc[0])), v = __builtin_fmaf(y, sc[1], x * sc[0]);
-      x = u;
-      y = v;
-    };
-    // fn(scale, inverse, codec) of the item's target.
-    auto store = [&](const It& it) __attribute__((always_inline)) {
-      if (it.kind == kNone) return;
-      constexpr bool kCodes = CACHE && KC::kBytes != C::kBytes;
-      const bool cached = kCodes && it.target > 0;
-      const float scale = it.target == 2 ? a.value_scale : a.key_scale;
-      const float inverse = it.target == 2 ? a.value_inverse : a.key_inverse;
-      const f32x2* sc = table + it.table + it.first;
-      float f[C::VEC];
-      C::unpack(it.w[0], f);
-      if (it.kind == kTurnVector) {
-        if constexpr (INTERLEAVED) {
+      const char* base = target == 0 ? a.q.from : target == 1 ? a.k.from : a.v.from;
+      const int64_t token = (target == 0 ? a.q.from_token : target == 1 ? a.k.from_token : a.v.from_token) * C::kBytes;
+      const char* p = base + t0 * token + from;
+      u32x4 w[TOKENS][INTERLEAVED ? 1 : 2];
+      float x[TOKENS], y[TOKENS];
+      const int apart = (INTERLEAVED ? 1 : a.half) * C::kBytes;  // from a to b of a pair
 #pragma unroll
-          for (int i = 0; i < It::kPairs; ++i) {
-            if (!WHOLE || !CACHE || it.target < 2) turn(f[2 * i], f[2 * i + 1], sc[i]);
-          }
-        } else {
-          float g[C::VEC];
-          C::unpack(it.w[1], g);
-#pragma unroll
-          for (int i = 0; i < C::VEC; ++i) {
-            if (!WHOLE || !CACHE || it.target < 2) turn(f[i], g[i], sc[i]);
-          }
-          if (cached) {
-            KC::vector(g, it.to + (int64_t)a.half * KC::kBytes, scale, inverse);
+      for (int u = 0; u < TOKENS; ++u) {
+        if (u < count && kind != kNone) {
+          if (WHOLE || kind == kTurnVector || kind == kCopyVector) {
+            w[u][0] = load16<NT>(p);
+            if constexpr (!INTERLEAVED) {
+              if (WHOLE || kind == kTurnVector) w[u][1] = load16<NT>(p + apart);
+            }
           } else {
-            QC::vector(g, it.to + (int64_t)a.half * C::kBytes, 0.0f, 0.0f);
+            x[u] = C::load1(p, 0);
+            if (kind == kTurnPair) y[u] = C::load1(p + apart, 0);
           }
         }
-        if (cached) {
-          KC::vector(f, it.to, scale, inverse);
-        } else {
-          QC::vector(f, it.to, 0.0f, 0.0f);
-        }
-        return;
+        p += token;
       }
-      if constexpr (!WHOLE) {
-        if (it.kind == kCopyVector) {
-          if (cached) {
-            KC::vector(f, it.to, scale, inverse);
+      if (i0 == begin) {
+        for (int j = (int)threadIdx.x; j < count * a.half; j += threads) {
+          const int t = j / a.half;
+          const f32x2 sc = sin_cos((double)a.positions[t0 + t], a.frequencies[j - t * a.half]);
+          table[j] = (f32x2){sc[0] * a.sine_sign, sc[1] * a.factor};
+        }
+        lds_written();
+      }
+#pragma unroll
+      for (int u = 0; u < TOKENS; ++u) {
+        if (u >= count) break;
+        // Of this token: the same in all lanes.
+        const int64_t t = t0 + u;
+        const int64_t slot = CACHE ? a.slots[t] : t;
+        const bool has_slot = !CACHE || (slot >= 0 && slot < a.slot_count);  // else k and v are not written
+        char* const to_q = q_to + t * a.q.to_token * C::kBytes;
+        const int64_t row = (has_slot ? slot : 0) * cache_row;
+        const f32x2* const sc = table + u * a.half + first;
+        auto turn = [&](float& c, float& d, const f32x2& by) __attribute__((always_inline)) {
+          const float m = __builtin_fmaf(c, by[1], -(d * by[0])), n = __builtin_fmaf(d, by[1], c * by[0]);
+          c = m;
+          d = n;
+        };
+        // fn(where a token's are, whether as codes, their scale): where the lane's results go.
+        auto to_target = [&](auto&& fn) __attribute__((always_inline)) {
+          if (kind == kNone || (target > 0 && !has_slot)) return;
+          if (target == 0) {
+            fn(to_q, std::false_type{}, 1.0f, 1.0f);
+          } else if (!CACHE || target == 1) {
+            fn(k_to + row, std::bool_constant<kCodes>{}, key_scale, key_inverse);
           } else {
-            QC::vector(f, it.to, 0.0f, 0.0f);
+            fn(v_to + row, std::bool_constant<kCodes>{}, value_scale, value_inverse);
           }
-          return;
-        }
-        float x = it.a, y = it.b;
-        const bool pair = it.kind == kTurnPair;
-        if (pair) turn(x, y, *sc);
-        const int64_t apart = INTERLEAVED ? 1 : a.half;
-        if (cached) {
-          KC::one(x, it.to, scale, inverse);
-          if (pair) KC::one(y, it.to + apart * KC::kBytes, scale, inverse);
-        } else {
-          C::store1(it.to, 0, x);
-          if (pair) C::store1(it.to, apart, y);
+        };
+        if (WHOLE || kind == kTurnVector || kind == kCopyVector) {
+          float f[C::VEC], g[C::VEC];
+          C::unpack(w[u][0], f);
+          const bool turned = WHOLE ? !CACHE || target < 2 : kind == kTurnVector;
+          const bool both = !INTERLEAVED && (WHOLE || kind == kTurnVector);
+          if constexpr (INTERLEAVED) {
+            if (turned) {
+#pragma unroll
+              for (int j = 0; j < kPairs; ++j) turn(f[2 * j], f[2 * j + 1], sc[j]);
+            }
+          } else {
+            C::unpack(w[u][1], g);
+            if (turned) {
+#pragma unroll
+              for (int j = 0; j < C::VEC; ++j) turn(f[j], g[j], sc[j]);
+            }
+          }
+          to_target([&](char* at, auto codes, float scale, float inverse) __attribute__((always_inline)) {
+            if constexpr (decltype(codes)::value) {
+              KC::vector(f, at + to, scale, inverse);
+              if (both) KC::vector(g, at + to + a.half * KC::kBytes, scale, inverse);
+            } else if constexpr (NT) {
+              const RowBuf<true, kPolSC1 | kPolNT> row(at, 0x7fffffffu);
+              row.st16(C::pack(f), (uint32_t)to);
+              if (both) row.st16(C::pack(g), (uint32_t)to + (uint32_t)apart);
+            } else {
+              Plain<C>::vector(f, at + to, 0.0f, 0.0f);
+              if (both) Plain<C>::vector(g, at + to + apart, 0.0f, 0.0f);
+            }
+          });
+        } else if constexpr (!WHOLE) {
+          float c = x[u], d = y[u];
+          const bool pair = kind == kTurnPair;
+          if (pair) turn(c, d, *sc);
+          to_target([&](char* at, auto codes, float scale, float inverse) __attribute__((always_inline)) {
+            if constexpr (decltype(codes)::value) {
+              KC::one(c, at + to, scale, inverse);
+              if (pair) KC::one(d, at + to + (INTERLEAVED ? 1 : a.half), scale, inverse);
+            } else {
+              C::store1(at + to, 0, c);
+              if (pair) C::store1(at + to + apart, 0, d);
+            }
+          });
         }
       }
-    };
-
-    It items[kInFlight];
-#pragma unroll
-    for (int u = 0; u < kInFlight; ++u) load(begin + (int)threadIdx.x + u * kThreads, items[u]);
-    for (int i = threadIdx.x; i < count * a.half; i += kThreads) {
-      const int t = i / a.half;
-      const f32x2 sc = sin_cos((double)a.positions[t0 + t], a.frequencies[i - t * a.half]);
-      table[i] = (f32x2){sc[0] * a.sine_sign, sc[1] * a.factor};
     }
-    __syncthreads();
-    for (int i = begin + (int)threadIdx.x;;) {
-#pragma unroll
-      for (int u = 0; u < kInFlight; ++u) store(items[u]);
-      i += kInFlight * kThreads;
-      if (i - (int)threadIdx.x >= end) break;
-#pragma unroll
-      for (int u = 0; u < kInFlight; ++u) load(i + u * kThreads, items[u]);
-    }
-    __syncthreads();  // the table is read
+    if (id + gridDim.x < groups) __syncthreads();  // the table is read
   }
 }
 
-// Tokens a workgroup takes and workgroups a token's items are spread over.
-template <class C, class KC, bool INTERLEAVED, bool CACHE, bool WHOLE, bool NT>
-int32_t run(Args a, bool copy_q, int of_token, hipStream_t st) {
-  const int64_t room = a.half > 0 ? kThreads / a.half : 8;
-  int64_t each = a.tokens / 1024;
-  each = each < 1 ? 1 : each;
-  const int64_t most = room < 1 ? 1 : room;
-  a.block_tokens = (int)(each < most ? each : most);
-  const int64_t groups = (a.tokens + a.block_tokens - 1) / a.block_tokens;
-  a.slices = groups < 512 ? (of_token * a.block_tokens + kThreads - 1) / kThreads : 1;
-  const int64_t blocks = groups * a.slices;
-  const unsigned grid = (unsigned)(blocks < (int64_t(1) << 22) ? blocks : (int64_t(1) << 22));
-  const size_t lds = (size_t)a.block_tokens * a.half * sizeof(f32x2);
-  rope_at<C, KC, INTERLEAVED, CACHE, WHOLE, NT><<<grid, kThreads, lds, st>>>(a, copy_q ? 1 : 0);
+template <class C, class KC, bool INTERLEAVED, bool CACHE, bool WHOLE, bool NT, int TOKENS>
+int32_t run(const Args& a, bool copy_q, int of_token, hipStream_t st) {
+  const int64_t groups = (a.tokens + TOKENS - 1) / TOKENS;
+  // A thread for each of a token's pieces; where tokens are few, workgroups of 128 threads for them.
+  const int most = groups < 256 ? kFewThreads : kMaxThreads;
+  const int threads = (of_token + 63) / 64 * 64 < most ? (of_token + 63) / 64 * 64 : most;
+  const int slices = groups < 256 ? (of_token + threads - 1) / threads : 1;
+  const dim3 grid((unsigned)(groups < kMaxGroups ? groups : kMaxGroups), (unsigned)slices);
+  rope_at<C, KC, INTERLEAVED, CACHE, WHOLE, NT, TOKENS>
+      <<<grid, threads, (size_t)TOKENS * a.half * sizeof(f32x2), st>>>(a, copy_q ? 1 : 0);
   return launch_status();
 }
 
@@ -331,13 +307,18 @@ int32_t by_shape(const Args& a, bool copy_q, hipStream_t st) {
   const int value = whole ? k.all() : a.dim / C::VEC + a.dim % C::VEC;
   const int64_t of_token = (int64_t)q.all() * a.q.heads + (int64_t)k.all() * a.k.heads +
                            (CACHE ? (int64_t)value * a.v.heads : 0);
-  // Item numbers of a workgroup's tokens are 32-bit.
-  if (of_token > (int64_t(1) << 21)) return (int32_t)hipErrorInvalidValue;
+  if (of_token > (int64_t(1) << 21)) return (int32_t)hipErrorInvalidValue;  // a token's pieces are counted in 32 bits
   if (of_token == 0) return (int32_t)hipSuccess;
-  if (!whole) return run<C, KC, INTERLEAVED, CACHE, false, false>(a, copy_q, (int)of_token, st);
+  if (!whole) return run<C, KC, INTERLEAVED, CACHE, false, false, 1>(a, copy_q, (int)of_token, st);
   const int64_t bytes = a.tokens * (a.q.heads + a.k.heads) * a.dim * C::kBytes;
-  if (bytes >= (int64_t(1) << 26)) return run<C, KC, INTERLEAVED, CACHE, true, true>(a, copy_q, (int)of_token, st);
-  return run<C, KC, INTERLEAVED, CACHE, true, false>(a, copy_q, (int)of_token, st);
+  // 32-bit offsets in a token, of tensors that go past the caches.
+  const auto reach = [&](const Heads& h) {
+    return h.to_head >= 0 && (h.heads * h.to_head + a.dim) * C::kBytes <= INT32_MAX;
+  };
+  if (bytes >= (int64_t(1) << 26) && reach(a.q) && reach(a.k)) {
+    return run<C, KC, INTERLEAVED, CACHE, true, true, 2>(a, copy_q, (int)of_token, st);
+  }
+  return run<C, KC, INTERLEAVED, CACHE, true, false, 1>(a, copy_q, (int)of_token, st);
 }
 
 bool sizes_ok(const Args& a) {
@@ -372,8 +353,8 @@ extern "C" int32_t launch_rope_at_fwd(const void* q, const void* k, void* q_out,
     if (!sizes_ok(a)) return (int32_t)hipErrorInvalidValue;
     const bool copy = !(q == q_out && k == k_out);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    return interleaved ? by_shape<C, Plain<C, false>, true, false>(a, copy, st)
-                       : by_shape<C, Plain<C, false>, false, false>(a, copy, st);
+    return interleaved ? by_shape<C, Plain<C>, true, false>(a, copy, st)
+                       : by_shape<C, Plain<C>, false, false>(a, copy, st);
   });
 }
 
@@ -420,6 +401,6 @@ extern "C" int32_t launch_rope_to_cache_fwd(const void* q, const void* k, const 
     };
     if (cache_dtype == kF8E4M3) return run_to(Codes<C, kF8E4M3>{});
     if (cache_dtype == kF8E5M2) return run_to(Codes<C, kF8E5M2>{});
-    return run_to(Plain<C, false>{});
+    return run_to(Plain<C>{});
   });
 }
