@@ -186,6 +186,9 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product(BlockArgs a) {
   constexpr int kAtQ = P::kLds, kAtS = kAtQ + Q::kLds, kSlot = kAtS + S::kLds, kLds = 2 * kSlot;
   constexpr int kAll = P::kLoads + Q::kLoads + 1;
   static_assert(FQ * 16 <= 128 && 128 % (FQ * 16) == 0);  // a wave's columns share a scale
+  // Columns that are multiplied while the others are read. Then the slot is free, and the loads of the step after
+  // the next go out between the products of the rest: at once they would hold each other up, with the matrix cores idle.
+  constexpr int kFirst = FQ / 2;
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
   __shared__ typename RowTiles<BP, NW * 64>::Shared shared;
 
@@ -207,20 +210,25 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product(BlockArgs a) {
   Q q(a.rows.w + ((int64_t)at.group * cols + tile.col) * ld, ld, tile.width, ld);
   S s(a, at, tile.col, tile.width);
   const LdsPtr slots = (LdsPtr)lds;
-  auto ask = [&](LdsPtr to) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < P::kLoads; ++i) {
+  // Load i of a step.
+  auto ask_one = [&](LdsPtr to, int i) __attribute__((always_inline)) {
+    if (i < P::kLoads) {
       P::place(to, i);
       place_ready();
       p.fetch(i);
-    }
-#pragma unroll
-    for (int i = 0; i < Q::kLoads; ++i) {
-      Q::place(to + kAtQ, i);
+    } else if (i < P::kLoads + Q::kLoads) {
+      Q::place(to + kAtQ, i - P::kLoads);
       place_ready();
-      q.fetch(i);
+      q.fetch(i - P::kLoads);
+    } else {
+      s.ask(to + kAtS);
     }
-    s.ask(to + kAtS);
+  };
+  auto ask = [&](LdsPtr to, int begin, int end) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = begin; i < end; ++i) ask_one(to, i);
+  };
+  auto advance = [&] {
     p.advance();
     q.advance();
   };
@@ -229,31 +237,65 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product(BlockArgs a) {
   const typename Q::template Lane<FQ> q_lane(slots + kAtQ, q0);
   const int lane = (int)threadIdx.x & 63;
   f32x4 acc[FP][FQ] = {};
-  ask(slots);
-  ask(slots + kSlot);
+  ask(slots, 0, kAll);
+  advance();
+  ask(slots + kSlot, 0, kAll);
+  advance();
   for (int t = 0; t < a.blocks; ++t) {
     const int slot = (t & 1) * kSlot;
+    const LdsPtr now = slots + slot;
     loads_landed<kAll>();
     meet();
     if (live) {
       BlockFragment<FX, EXACT> x[FP];
+      BlockFragment<FW, EXACT> w[FQ];
       float scale[FP];
-      const float of_cols = S::cols(slots + slot + kAtS, q0);
+      auto columns = [&](int j) __attribute__((always_inline)) {
+        w[j] = BlockFragment<FW, EXACT>(q_lane.fragment(j, 0, slot), q_lane.fragment(j, 1, slot));
+      };
+      columns(0);
 #pragma unroll
       for (int i = 0; i < FP; ++i) {
         x[i] = BlockFragment<FX, EXACT>(p_lane.fragment(i, 0, slot), p_lane.fragment(i, 1, slot));
-        scale[i] = S::row(slots + slot + kAtS, p0 + 16 * i + (lane & 15)) * of_cols;
       }
+      const float of_cols = S::cols(now + kAtS, q0);
+#pragma unroll
+      for (int i = 0; i < FP; ++i) scale[i] = S::row(now + kAtS, p0 + 16 * i + (lane & 15));
+      // Each product is added FP products later, when the matrix cores are done with it.
+      f32x4 part[FP];
 #pragma unroll
       for (int j = 0; j < FQ; ++j) {
-        const BlockFragment<FW, EXACT> w(q_lane.fragment(j, 0, slot), q_lane.fragment(j, 1, slot));
+        if (j < kFirst) {
+          columns(2 * j + 1);
+          if (2 * j + 2 < FQ) columns(2 * j + 2);
+        }
+        if (j == kFirst) {
+          lds_read();
+          meet();  // the slot has been read
+        }
+        if (j == 1) {
 #pragma unroll
-        for (int i = 0; i < FP; ++i) add_scaled(acc[i][j], block_mma<FX, FW, EXACT>(w, x[i]), scale[i]);
+          for (int i = 0; i < FP; ++i) scale[i] *= of_cols;
+        }
+#pragma unroll
+        for (int i = 0; i < FP; ++i) {
+          if (j > 0) add_scaled(acc[i][j - 1], part[i], scale[i]);
+          part[i] = block_mma<FX, FW, EXACT>(w[j], x[i]);
+          if (j >= kFirst) {
+            constexpr int kSpread = (FQ - kFirst) * FP;
+            const int n = (j - kFirst) * FP + i;
+            ask(now, n * kAll / kSpread, (n + 1) * kAll / kSpread);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < FP; ++i) add_scaled(acc[i][FQ - 1], part[i], scale[i]);
+    } else {
+      meet();
+      ask(now, 0, kAll);
     }
-    lds_read();
-    meet();
-    ask(slots + slot);
+    advance();
   }
   loads_landed();
   meet();  // nobody reads the slots any more, and nothing is on its way to them
