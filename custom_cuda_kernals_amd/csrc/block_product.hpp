@@ -567,6 +567,23 @@ int32_t launch_block_stream(const BlockArgs& a, hipStream_t st) {
   return launch_block_grid<FP * 16, FQ * 16>(block_stream<FX, FW, EXACT, FP, FQ, 4, DEPTH>, 256, a, st);
 }
 
+// Which kernel. bf16 results, us, weights from HBM; float32 ones go the same ways.
+// Streams read the weights once for each 16 or 32 rows, and are for few rows:
+//   where they make no more than two workgroups a CU. Streams of 32 rows against 64 x 64 tiles: 4096 x 4096, 128
+//   rows (512 workgroups) 12.8 and 14.2, 192 rows 17.4 and 14.5; 1408 x 2048, 256 rows (352) 7.8 and 8.7, 384 rows
+//   11.3 and 8.7; 14336 x 4096, 32 rows (448) 16.3 and 17.2, 48 rows 26.0 and 18.1;
+//   and for groups of 16 rows or less on average, whose rows are long enough for four waves: 8 of 14336 x 4096, of
+//   16 rows 90.8 and 93.1, of 24 rows 98.5 and 95.7; but 64 of 1408 x 2048, of 8 rows 40.5 and 29.2.
+// Of 16 rows and two fragments of columns, or one where that leaves CUs without (4096 x 4096, 16 rows 7.4 and 6.9).
+// Tiles of 256 x 256 where they are filled and enough for the CUs (against 128 x 128: 14336 x 4096, 1024 rows, 224
+// tiles 65.8 and 80.0, 512 rows, 112 tiles 63.3 and 45.8; 8 groups of 512 rows, 2048 x 2048, 160 by this count 31.5
+// and 22.5; 8 of 1024 rows, 288 37.4 and 42.4; 64 groups of 128 rows, 1408 x 2048 47.1 and 39.5, which are half empty;
+// 8 of 128 rows, 14336 x 4096 116 and 124; of 192 rows 133 and 151); not for float32 results, whose fragments are
+// twice as large.
+// Tiles of 64 x 64 where there would be fewer than 220 of 128 x 128 (against those: 8 groups of 128 rows, 2048 x 2048,
+// 208 by this count 12.2 and 15.4, of 192 rows, 272 16.1 and 15.6; 14336 x 4096, 192 rows, 224 35.3 and 24.2; 1408 x
+// 2048, 2048 rows, 187 14.8 and 14.5, 4096 rows, 363 25.2 and 19.7), and for groups that those leave three quarters empty (8 of 32 rows, 14336 x 4096 98.6
+// and 102; of 64 rows 116 and 108).
 template <int FX, int FW, bool EXACT>
 int32_t launch_block_linear(const BlockArgs& a, hipStream_t st) {
   const RowsArgs& r = a.rows;
@@ -578,19 +595,26 @@ int32_t launch_block_linear(const BlockArgs& a, hipStream_t st) {
   const bool whole = r.length % 16 == 0 && host_aligned(r.x, 16) && host_aligned(r.w, 16) && host_aligned(a.x_scale, 4) &&
                      host_aligned(a.w_scale, 4);
   if (!whole) return launch_block_tiles<FX, FW, EXACT, 2, 2, 2, 2, false>(a, st);
-  const bool one = r.groups == 1;
-  if (r.rows <= (one ? 16 : 8) * (int64_t)r.groups) {
-    const int64_t tiles = r.rows < r.groups ? r.rows : r.groups;
-    if (tiles * r.cols >= 256 * 32) return launch_block_stream<FX, FW, EXACT, 1, 2, 2>(a, st);
-    return launch_block_stream<FX, FW, EXACT, 1, 1, 2>(a, st);
+  const int64_t groups = r.groups, cols = r.cols;
+  // Of all groups, if they are equal.
+  const auto row_tiles = [&](int64_t height) {
+    const int64_t tiles = groups * ((r.rows + groups * height - 1) / (groups * height));
+    return tiles < r.rows ? tiles : r.rows;
+  };
+  if (r.rows <= 16 * groups) {
+    if (row_tiles(16) * ((cols + 31) / 32) <= 512 || a.blocks >= 32) {
+      if (row_tiles(16) * cols >= 256 * 32) return launch_block_stream<FX, FW, EXACT, 1, 2, 2>(a, st);
+      return launch_block_stream<FX, FW, EXACT, 1, 1, 2>(a, st);
+    }
+  } else if (row_tiles(32) * ((cols + 31) / 32) <= 512) {
+    return launch_block_stream<FX, FW, EXACT, 2, 2, 2>(a, st);
   }
-  if (r.rows <= 32 * (int64_t)r.groups) return launch_block_stream<FX, FW, EXACT, 2, 2, 2>(a, st);
   if constexpr (!EXACT) {
-    if (r.rows >= 128 * (int64_t)r.groups && (r.rows / 256 + r.groups / 2) * ((r.cols + 255) / 256) >= 150) {
+    if (r.rows >= 160 * groups && (r.rows / 256 + groups / 2) * ((cols + 255) / 256) >= 200) {
       return launch_block_tiles<FX, FW, EXACT, 4, 2, 4, 8, true>(a, st);
     }
   }
-  if ((r.rows / 128 + r.groups / 2 + 1) * ((r.cols + 127) / 128) >= 192) {
+  if (r.rows > 32 * groups && (r.rows / 128 + groups / 2 + 1) * ((cols + 127) / 128) >= 220) {
     return launch_block_tiles<FX, FW, EXACT, 2, 2, 4, 4, true>(a, st);
   }
   return launch_block_tiles<FX, FW, EXACT, 2, 2, 2, 2, true>(a, st);
