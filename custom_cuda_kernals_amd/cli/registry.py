@@ -238,6 +238,69 @@ def _t_mxfp4(device: str) -> Target:
                   (rows + n) * k // 32 * 17 + rows * n * 2)
 
 
+def _t_rope_at(device: str) -> Target:
+    import torch
+
+    from custom_cuda_kernals_amd.kernels import rope_at, rope_frequencies
+
+    g = _gen(device)
+    q, k = _rn((8192, 32, 128), torch.bfloat16, device, g), _rn((8192, 8, 128), torch.bfloat16, device, g)
+    positions = torch.randint(0, 131072, (8192,), device=device, generator=g)
+    frequencies, _ = rope_frequencies(128, 500000.0, device=device)
+
+    def eager():
+        angle = positions.double()[:, None] * frequencies
+        c, s = angle.cos().float()[:, None], angle.sin().float()[:, None]
+
+        def turn(t):
+            a, b = t.float().chunk(2, dim=-1)
+            return torch.cat([a * c - b * s, b * c + a * s], dim=-1).to(t.dtype)
+
+        return turn(q), turn(k)
+
+    return Target(lambda: rope_at(q, k, positions, frequencies), eager, "rope_at bf16 8192 tokens, 32 / 8 heads of 128",
+                  2 * (q.numel() + k.numel()) * 2 + 8192 * 8)
+
+
+def _t_paged_attention(device: str) -> Target:
+    import torch
+
+    from custom_cuda_kernals_amd.kernels import paged_attention
+
+    g = _gen(device)
+    b, context, page = 16, 4096, 16
+    q = _rn((b, 32, 128), torch.bfloat16, device, g)
+    keys, values = (_rn((b * context // page, page, 8, 128), torch.bfloat16, device, g) for _ in range(2))
+    table = torch.randperm(b * context // page, device=device, generator=g).view(b, -1)
+    lengths = torch.full((b,), context, device=device)
+
+    def eager():
+        k, v = (c[table].flatten(1, 2).transpose(1, 2).repeat_interleave(4, 1) for c in (keys, values))
+        return torch.nn.functional.scaled_dot_product_attention(q.unsqueeze(2), k, v).squeeze(2)
+
+    return Target(lambda: paged_attention(q, keys, values, table, lengths), eager,
+                  "paged_attention bf16 16 sequences of 4096, 32 / 8 heads of 128", 2 * keys.numel() * 2 + 2 * q.numel() * 2)
+
+
+def _t_fp8_linear(device: str) -> Target:
+    import torch
+
+    from custom_cuda_kernals_amd.fp8_format import dequantize
+    from custom_cuda_kernals_amd.kernels import fp8_block_linear, fp8_quant
+
+    g = _gen(device)
+    rows, n, k = 16, 14336, 4096
+    x = fp8_quant(_rn((rows, k), torch.bfloat16, device, g), "e4m3", "group")
+    w = fp8_quant(_rn((n, k), torch.bfloat16, device, g), "e4m3", "block")
+    values = dequantize(*w, "block", torch.bfloat16)
+
+    def eager():
+        return dequantize(*x, "group", torch.bfloat16) @ values.t()
+
+    return Target(lambda: fp8_block_linear(*x, *w), eager, "fp8_block_linear [16, 4096] x [14336, 4096]",
+                  (rows + n) * k + rows * n * 2)
+
+
 _CSRC = "custom_cuda_kernals_amd/csrc/"
 
 REGISTRY: dict[str, OpSpec] = {
@@ -414,6 +477,53 @@ REGISTRY: dict[str, OpSpec] = {
             test_files=("tests/test_mxfp4_gpu.py", "tests/test_expert_layer_gpu.py",
                         "tests/test_expert_products_use_gpu.py", "tests/test_products_cpu.py"),
             bench_ops=(), build_target=_t_mxfp4),
+        OpSpec(
+            id="rope_at", number=11, title="Rotary positions of any kind, and their gradient",
+            purpose="RoPE at given positions: half-split or interleaved pairs, part of a head, scaled for long contexts.",
+            formula="a' = s (a cos - b sin), b' = s (b cos + a sin), angle = position * frequency in float64; "
+                    "the gradient turns back",
+            dtypes=("float32", "float16", "bfloat16"),
+            memory_profile="HBM-bound: q and k once each way.",
+            design=("no tables: a workgroup's threads make the angles of its tokens while its vectors are on their way",
+                    "a thread has the same pieces of each of its workgroup's tokens",
+                    "large tensors: stores that go on from the caches at once"),
+            target="within 2^-21 of the pair's size and one rounding of the float64 formula",
+            reference=("an addition",), python_api=("rope_at", "rope_frequencies"),
+            c_entry_points=("launch_rope_at_fwd",), sources=(_CSRC + "rotary.hip",),
+            test_files=("tests/test_rotary_gpu.py", "tests/test_decode_use_gpu.py", "tests/test_decode_cpu.py"),
+            bench_ops=(), build_target=_t_rope_at),
+        OpSpec(
+            id="paged_attention", number=12, title="A paged key-value cache, and attention of one token over it",
+            purpose="Decode: write turned keys and values into pages, attend over each sequence's pages.",
+            formula="softmax(scale q . k) v over a sequence's positions; lse; key_cache[slot] = rope(k) / key_scale",
+            dtypes=("float32", "float16", "bfloat16", "FP8 caches"),
+            memory_profile="HBM-bound: the keys and values of every position once.",
+            design=("a wave a part of a sequence's positions and a key-value head, all its query heads at once",
+                    "keys and values straight from memory into LDS, two steps or more ahead",
+                    "parts of one length over all sequences, found on the GPU; a second launch joins them",
+                    "16-bit weights in two parts, so that the output's own rounding is the largest"),
+            target="sums in float32; the same bits from every launch",
+            reference=("an addition",), python_api=("rope_to_cache", "paged_attention"),
+            c_entry_points=("launch_rope_to_cache_fwd", "launch_paged_attention_fwd"),
+            sources=(_CSRC + "paged_attention.hip", _CSRC + "rotary.hip"),
+            test_files=("tests/test_paged_attention_gpu.py", "tests/test_rotary_gpu.py", "tests/test_decode_use_gpu.py",
+                        "tests/test_decode_cpu.py"),
+            bench_ops=(), build_target=_t_paged_attention),
+        OpSpec(
+            id="fp8_linear", number=13, title="Products of FP8 with a scale for each block of 128",
+            purpose="Linear layers on what fp8_quant writes in groups or 128 x 128 tiles, dense or grouped by expert.",
+            formula="y[s][n] = sum over blocks b of sx[s][b] sw[n / 128][b] sum_{k in b} x[s][k] w[n][k]",
+            dtypes=("fp8 e4m3 and e5m2", "results float32, float16, bfloat16"),
+            memory_profile="few rows: HBM-bound (the weights, once); many: bound by the matrix cores.",
+            design=("one matrix instruction a block of 128, its sums scaled into the tile's by the vector units",
+                    "float32 results: exact products, as bfloat16",
+                    "tiles and rings as grouped_linear's"),
+            target="block sums scaled in float32, one rounding; the same bits from every launch",
+            reference=("an addition",), python_api=("fp8_block_linear", "fp8_quant"),
+            c_entry_points=("launch_fp8_block_linear_fwd", "launch_fp8_quant_group_fwd"),
+            sources=(_CSRC + "fp8_linear.hip", _CSRC + "block_product.hpp", _CSRC + "tile_product.hpp"),
+            test_files=("tests/test_fp8_linear_gpu.py", "tests/test_decode_use_gpu.py", "tests/test_decode_cpu.py"),
+            bench_ops=(), build_target=_t_fp8_linear),
     ]
 }
 

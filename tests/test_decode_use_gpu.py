@@ -269,3 +269,14 @@ def test_config_of_another_head_dim():
         blk.prefill(x[:, :32].contiguous(), cache, *cache.advance(32))
         y = blk.decode(x[:, 32:].contiguous(), cache, *cache.advance(1))
         assert _off(y, blk(x)[:, 32:], x[:, 32:]) < 0.02
+
+
+@pytest.mark.parametrize("op_id", ["rope_at", "paged_attention", "fp8_linear"])
+def test_cli_targets(op_id):
+    """The developer CLI's calls agree with their eager formulas: bf16 values, rounded once or twice each."""
+    from custom_cuda_kernals_amd.cli.registry import REGISTRY
+
+    target = REGISTRY[op_id].build_target("cuda")
+    got, want = target.kernel(), target.eager()
+    for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+        assert a.shape == b.shape and (a.float() - b.float()).norm() < 0.01 * b.float().norm()
