@@ -186,8 +186,10 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product(BlockArgs a) {
   constexpr int kAtQ = P::kLds, kAtS = kAtQ + Q::kLds, kSlot = kAtS + S::kLds, kLds = 2 * kSlot;
   constexpr int kAll = P::kLoads + Q::kLoads + 1;
   static_assert(FQ * 16 <= 128 && 128 % (FQ * 16) == 0);  // a wave's columns share a scale
-  // Columns that are multiplied while the others are read. Then the slot is free, and the loads of the step after
-  // the next go out between the products of the rest: at once they would hold each other up, with the matrix cores idle.
+  // Columns that are multiplied while the others are read. Then the waves meet, once a step: this slot is free, and
+  // the next one has landed. The loads of the step after that go out between the products of the rest: at once they
+  // would hold each other up, with the matrix cores idle. 8192 rows, 14336 x 4096, us: 420; at once 460, with a meeting
+  // of its own for each of the two 445.
   constexpr int kFirst = FQ / 2;
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
   __shared__ typename RowTiles<BP, NW * 64>::Shared shared;
@@ -241,11 +243,11 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product(BlockArgs a) {
   advance();
   ask(slots + kSlot, 0, kAll);
   advance();
+  loads_landed<kAll>();
+  meet();
   for (int t = 0; t < a.blocks; ++t) {
     const int slot = (t & 1) * kSlot;
     const LdsPtr now = slots + slot;
-    loads_landed<kAll>();
-    meet();
     if (live) {
       BlockFragment<FX, EXACT> x[FP];
       BlockFragment<FW, EXACT> w[FQ];
@@ -271,7 +273,8 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product(BlockArgs a) {
         }
         if (j == kFirst) {
           lds_read();
-          meet();  // the slot has been read
+          loads_landed();
+          meet();  // this slot has been read, and the next has landed
         }
         if (j == 1) {
 #pragma unroll
@@ -292,6 +295,7 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product(BlockArgs a) {
 #pragma unroll
       for (int i = 0; i < FP; ++i) add_scaled(acc[i][FQ - 1], part[i], scale[i]);
     } else {
+      loads_landed();
       meet();
       ask(now, 0, kAll);
     }
