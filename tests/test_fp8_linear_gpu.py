@@ -283,3 +283,26 @@ def test_same_bits_every_time():
         args = [t.cuda() for t in _random(rows, 3000, 512, None, "e4m3", "e4m3", False, 30)]
         first = K.fp8_block_linear(*args)
         assert all(torch.equal(K.fp8_block_linear(*args), first) for _ in range(3))
+
+
+@pytest.mark.parametrize("out", [torch.float16, torch.bfloat16], ids=IDS[1:])
+@pytest.mark.parametrize("tall", [False, True], ids=["group", "block"])
+@pytest.mark.parametrize("rows,n,k", [(4100, 3700, 272), (2100, 8200, 2064), (4352, 3590, 128)])
+def test_large_tiles(rows, n, k, tall, out):
+    _check(*_random(rows, n, k, None, "e5m2", "e4m3", tall, k), out=out, tall=tall)
+
+
+def test_large_tiles_of_groups():
+    offsets = torch.tensor([3, 1000, 1000, 2100, 3001, 3002, 4400])
+    got = _check(*_random(4407, 3700, 400, 6, "e4m3", "e5m2", False, 40), offsets=offsets)
+    assert (got[:3] == 0).all() and (got[4400:] == 0).all()
+
+
+@pytest.mark.parametrize("rows,n", [(3, 70), (20, 300), (150, 300), (3000, 3300), (4100, 3700)])
+def test_infinities_and_nan_of_16_bit_results(rows, n):
+    x, xs, w, ws = _random(rows, n, 400, None, "e5m2", "e4m3", False, 41)
+    x[rows // 2, 131], x[0, 399] = float("inf"), float("nan")
+    w[n // 3, 17] = float("nan")
+    bad = ~K.fp8_block_linear(x.cuda(), xs.cuda(), w.cuda(), ws.cuda()).isfinite()
+    assert bad[0].all() and bad[rows // 2].all() and bad[:, n // 3].all()
+    assert bad.sum() == 2 * n + rows - 2

@@ -273,3 +273,74 @@ def test_cache_of_strided_slices():
     want = K.rope_to_cache(q.contiguous(), k.contiguous(), v.contiguous(), *caches[:2], slots, positions, frequencies)
     got = K.rope_to_cache(q, k, v, *caches[2:], slots, positions, frequencies, inplace=True)
     assert torch.equal(got, want) and torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+
+
+# ---------------------------------------------------------------------------
+# Many tokens: the same bits as of small calls.
+# ---------------------------------------------------------------------------
+
+def _in_chunks(fn, count, *tensors):
+    parts = [fn(*(t[i:i + count] for t in tensors)) for i in range(0, len(tensors[0]), count)]
+    return [torch.cat(p) for p in zip(*parts)]
+
+
+LARGE = [(torch.bfloat16, 4099, 56, 8, 128, 128, "half"), (torch.bfloat16, 4099, 56, 8, 128, 128, "interleaved"),
+         (torch.float32, 3001, 24, 24, 128, 64, "half"), (torch.float16, 16385, 32, 1, 64, 64, "interleaved")]
+
+
+@pytest.mark.parametrize("dtype,tokens,heads,kv,dim,rotary,layout", LARGE)
+def test_large(dtype, tokens, heads, kv, dim, rotary, layout):
+    frequencies, _ = K.rope_frequencies(rotary, 500000.0)
+    g = torch.Generator("cuda").manual_seed(50)
+    q, k = (torch.randn((tokens, n, dim), generator=g, device="cuda").to(dtype) for n in (heads, kv))
+    positions = _positions((tokens,), 1 << 20, 51).cuda()
+    for inverse in (False, True):
+        def rope(q, k, p, **how):
+            return K.rope_at(q, k, p, frequencies, layout=layout, scale=1.25, inverse=inverse, **how)
+        want = _in_chunks(rope, 500, q, k, positions)
+        assert all(torch.equal(a, b) for a, b in zip(rope(q, k, positions), want))
+    wide = torch.full((tokens, heads + kv + 3, dim), 2.0, dtype=dtype, device="cuda")
+    wide[:, :heads], wide[:, heads:heads + kv] = q, k
+    rope(wide[:, :heads], wide[:, heads:heads + kv], positions, inplace=True)
+    assert torch.equal(wide[:, :heads], want[0]) and torch.equal(wide[:, heads:heads + kv], want[1])
+    assert (wide[:, heads + kv:] == 2.0).all()
+
+
+@pytest.mark.parametrize("cache", ["same", "e4m3", "e5m2"])
+@pytest.mark.parametrize("dtype,tokens,heads,kv,dim,rotary,layout", LARGE[:3])
+def test_large_to_cache(dtype, tokens, heads, kv, dim, rotary, layout, cache):
+    frequencies, _ = K.rope_frequencies(rotary, 500000.0)
+    g = torch.Generator("cuda").manual_seed(52)
+    q, k, v = (torch.randn((tokens, n, dim), generator=g, device="cuda").to(dtype) for n in (heads, kv, kv))
+    positions, page = _positions((tokens,), 1 << 20, 53).cuda(), 7
+    pages = tokens // page + 3
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(54))[:tokens].cuda()
+    slots[[5, tokens - 1]] = torch.tensor([-1, pages * page], device="cuda")
+    kind = dtype if cache == "same" else FP8[cache]
+    raw = dtype if cache == "same" else torch.uint8
+    caches = [torch.full((pages, page, kv, dim), 3.0, device="cuda").to(kind) for _ in range(4)]
+    scales = {} if cache == "same" else {"key_scale": 0.02, "value_scale": 0.3}
+
+    def rope(keys, values, inplace=False):
+        return lambda q, k, v, s, p: [K.rope_to_cache(q, k, v, keys, values, s, p, frequencies, layout=layout,
+                                                      inplace=inplace, **scales)]
+    want, = _in_chunks(rope(*caches[:2]), 500, q, k, v, slots, positions)
+    assert torch.equal(rope(*caches[2:])(q, k, v, slots, positions)[0], want)
+    assert all(torch.equal(caches[i].view(raw), caches[i + 2].view(raw)) for i in (0, 1))
+    for c in caches[2:]:
+        c.view(raw).zero_()
+    same, = rope(*caches[2:], inplace=True)(q, k, v, slots, positions)
+    assert same is q and torch.equal(q, want)
+    written = slots[(slots >= 0) & (slots < pages * page)]
+    assert all(torch.equal(caches[i].view(raw).flatten(0, 1)[written], caches[i + 2].view(raw).flatten(0, 1)[written])
+               for i in (0, 1))
+
+
+def test_more_tokens_than_workgroups():
+    frequencies, _ = K.rope_frequencies(6)
+    tokens = (1 << 21) + 5
+    g = torch.Generator("cuda").manual_seed(55)
+    q = torch.randn((tokens, 1, 6), generator=g, device="cuda").half()
+    positions = torch.randint(0, 1 << 17, (tokens,), generator=g, device="cuda")
+    want = _in_chunks(lambda q, p: K.rope_at(q, q[:, :0], p, frequencies), 1 << 20, q, positions)[0]
+    assert torch.equal(K.rope_at(q, q[:, :0], positions, frequencies)[0], want)
