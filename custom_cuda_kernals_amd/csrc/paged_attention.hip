@@ -56,7 +56,7 @@ using i32x2 = int __attribute__((ext_vector_type(2)));
 // row: 16 bytes.
 struct Bf16 {
   using Codec = CodecBF16;
-  static constexpr int kBytes = 2;
+  static constexpr int kBytes = 2, kLift = 0;
   __device__ static f32x4 mma(const u32x4& a, const u32x4& b, const f32x4& c) { return ElemBF16::mma(a, b, c, 0, 0); }
   __device__ static uint32_t pack(float lo, float hi) { return pack2_bf16(lo, hi); }
   __device__ static float low(uint32_t w) { return bf16_lo(w); }
@@ -64,7 +64,8 @@ struct Bf16 {
 };
 struct F16 {
   using Codec = CodecF16;
-  static constexpr int kBytes = 2;
+  // P times 2^7: with kSlack 2^15 at most, and what a long tail of small ones has keeps its bits down to 2^-31.
+  static constexpr int kBytes = 2, kLift = 7;
   __device__ static f32x4 mma(const u32x4& a, const u32x4& b, const f32x4& c) { return ElemF16::mma(a, b, c, 0, 0); }
   __device__ static uint32_t pack(float lo, float hi) { return pack2_f16(lo, hi); }
   __device__ static float low(uint32_t w) { return f16_lo(w); }
@@ -72,7 +73,7 @@ struct F16 {
 };
 struct F32 {
   using Codec = CodecF32;
-  static constexpr int kBytes = 4;
+  static constexpr int kBytes = 4, kLift = 0;
   __device__ static f32x4 mma(const u32x4& a, const u32x4& b, const f32x4& c) { return ElemF32::mma(a, b, c, 0, 0); }
 };
 
@@ -375,7 +376,8 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
 
   constexpr int kOut = DIM / 16;
   f32x4 out[kOut] = {};
-  float top = -__builtin_inff(), base = 0.0f, sum = 0.0f;  // base: top, or 0 while there is none
+  // P is taken by base: top - kLift, or 0 while there is none.
+  float top = -__builtin_inff(), base = 0.0f, sum = 0.0f;
   auto step = [&](const LdsPtr slot, uint32_t seen) __attribute__((always_inline)) {
     constexpr uint32_t kEvery = kStep == 32 ? 0xffffffffu : 0xffffu;
     const bool all = (seen & kEvery) == kEvery;
@@ -431,8 +433,8 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
       most = __builtin_fmaxf(most, __shfl_xor(most, 16));
       most = __builtin_fmaxf(most, __shfl_xor(most, 32));
       const float now = __builtin_fmaxf(top, most);
-      base = now == -__builtin_inff() ? 0.0f : now;
-      const float keep = __builtin_amdgcn_exp2f(top - base);
+      const float keep = __builtin_amdgcn_exp2f(top - (now == -__builtin_inff() ? 0.0f : now));
+      base = now == -__builtin_inff() ? 0.0f : now - T::kLift;
       top = now;
       sum *= keep;
 #pragma unroll
@@ -532,6 +534,7 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
   }
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
+  top -= T::kLift;  // the sums' power of two from here on
 
   if (col >= heads) return;
   const int in_sequence = kv * group + head0 + col;
@@ -564,6 +567,7 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
 
 constexpr int kMaxParts = 1024;  // of all sequences, or twice as many as there are of them
 constexpr int64_t kMaxPositions = int64_t(1) << 30;  // of a sequence: a step past the last is still an int
+constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
 constexpr int kMaxCut = 2048;  // sequences: beyond it each is one part, so that nobody reads so many lengths
 
 // The sums of a sequence's parts, a head a workgroup. A thread has four elements of every
@@ -646,7 +650,8 @@ int parts_of(int64_t sequences, int64_t units, int64_t positions, int64_t dim, i
   const int64_t limit = 2 * sequences > kMaxParts ? 2 * sequences : kMaxParts;
   parts = parts < limit ? parts : limit;
   const int64_t most = sequences * ((positions + kMinPart - 1) / kMinPart) + sequences;  // of the shortest parts
-  return (int)(parts < most ? parts : most);
+  parts = parts < most ? parts : most;
+  return parts * units <= kMaxBlocks ? (int)parts : 0;  // so many heads fill the card by themselves
 }
 
 template <class T, class S>
@@ -746,7 +751,6 @@ extern "C" int32_t launch_paged_attention_fwd(const void* q, const void* key_cac
   a.score_scale = scale * key_scale * kLog2e;
   a.value_scale = value_scale;
   const int64_t blocks = (a.parts > 0 ? a.parts : sequences) * units;
-  if (blocks > (int64_t(1) << 24) - 1) return (int32_t)hipErrorInvalidValue;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {
     case kF32: return run_cache<F32>(a, blocks, cache_dtype, st);

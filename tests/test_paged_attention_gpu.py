@@ -234,3 +234,39 @@ def test_same_bits_every_time():
     for _ in range(5):
         again = K.paged_attention(*case, return_lse=True)
         assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+
+
+@pytest.mark.parametrize("cache", [None, torch.float8_e4m3fn], ids=["same", "e4m3"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_many_small_probabilities(dtype, cache):
+    """One position of probability almost 1 and 2^18 of 2^-26 of it, which float16 has not got: 2^-8 of the sum
+    together. Values 1 and 2, so out is 1 + 2^-8 / (1 + 2^-8) and each small probability counts."""
+    n = (1 << 18) + 1
+    q = torch.full((1, 1, 16), 2.0, dtype=dtype)
+    keys = torch.zeros((n, 1, 1, 16), dtype=dtype)
+    values = torch.full((n, 1, 1, 16), 2.0, dtype=dtype)
+    for at in (0, n // 2, n - 1):
+        keys[:], values[:] = 0.0, 2.0
+        keys[at], values[at] = 1.0, 1.0  # its score: 32 scale
+        args = q, keys.to(cache or dtype), values.to(cache or dtype), torch.arange(n)[None], torch.tensor([n])
+        out, lse = K.paged_attention(*(t.cuda() for t in args), scale=26 * np.log(2.0) / 32, return_lse=True)
+        tail = 2.0 ** -26 * (n - 1)
+        want = 1.0 + tail / (1.0 + tail)
+        # The exponent 26 in float32 is a relative 2^-19 of the tail; its n terms' sum, in parts of no more than 2^13
+        # and these of no more than 2^10, 2^-10 of it at most; as float16, lifted by 2^7, its terms are 2^-19 and off
+        # by 2^-25 at most: 2^-6. So less than 2^-5 of the tail, 2^-13, and the output's rounding.
+        assert (out.double().cpu() - want).abs().max() <= 2.0 ** -13 + want * torch.finfo(dtype).eps / 2
+        # lse = 26 log 2 + log(1 + tail): those of the sum's errors, and float32's own of 18.02
+        assert abs(float(lse.cpu()) - (26 * np.log(2.0) + np.log1p(tail))) <= 2.0 ** -13 + 18.1 * 2.0 ** -22
+
+
+def test_most_heads():
+    """2^23 query heads in all: too many workgroups for parts of the sequences."""
+    b, heads = 2048, 4096
+    g = torch.Generator("cuda").manual_seed(60)
+    q = torch.randn((b, heads, 16), generator=g, device="cuda").half()
+    keys, values = (torch.randn((3, 16, heads, 16), generator=g, device="cuda").half() for _ in range(2))
+    table, lengths = torch.tensor([[2, 0, 1]]).repeat(b, 1), torch.arange(b) % 49
+    out, lse = K.paged_attention(q, keys, values, table.cuda(), lengths.cuda(), return_lse=True)
+    some = torch.tensor([0, 1, 48, 1000, b - 1])
+    _check(q[some].cpu(), keys.cpu(), values.cpu(), table[some], lengths[some], got=(out[some], lse[some]))
