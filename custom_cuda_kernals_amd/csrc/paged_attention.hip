@@ -15,12 +15,17 @@
 // one product to the other inside the lane. 16-bit P is split in two parts, high and low:
 // rounded once, it would add an error as large as that of the output's own rounding.
 //
-// Bound by HBM: reading keys and values once. The sequences are cut into parts of one
-// length, as many as fill the card; a workgroup is one wave with one part of one key-value
-// head, and the parts' sums meet in a second launch. The lengths are on the GPU, so each
-// workgroup finds its part itself, from the sum of all lengths. Keys and values go straight from memory to LDS,
-// whole rows at a time, into a ring of two steps: a step is on its way while the one
-// before is worked on, without registers or other waves to wait for.
+// Bound by HBM: reading keys and values once. A wave works alone, on positions of one
+// sequence and one key-value head. Short contexts have a wave or a workgroup's few waves
+// for each; long ones are cut into parts of one length, as many as fill the card, whose
+// sums meet in a second launch. The lengths are on the GPU, so each workgroup finds its
+// part itself, from the sum of all lengths. Keys and values go straight from memory to
+// LDS, whole rows at a time, into a ring of two steps or more: steps are on their way
+// while one is worked on, without registers or other waves to wait for.
+//
+// 8 key-value heads of 128: 64 sequences of up to 8192 positions, bf16, 1.08 GB, 192 us,
+// 5.6 TB/s (a copy reaches 5.2); two of 131072, e4m3, 0.54 GB, 106 us, 5.1 TB/s; 1024 of up
+// to 512 180 us, 5.9 TB/s; one of 700 10.4 us, where steps are waited for.
 #include "tile_product.hpp"
 
 namespace cck {
@@ -118,7 +123,8 @@ struct FromCodes {
 
 // The positions of a sequence that are seen: [lo, lo + seen).
 struct Seen {
-  int lo, seen;
+  int lo = 0, seen = 0;
+  __device__ Seen() = default;
   __device__ Seen(const AttentionArgs& a, int sequence) {
     const int64_t most = (int64_t)a.table_width * a.page;
     int64_t n = a.lengths[sequence];
@@ -138,11 +144,17 @@ __device__ inline int* notes_of(const AttentionArgs& a) {
 // the wave calls.
 struct Cut {
   int each, run, mine, before, all;  // sequences of a run; parts of the lane's, before them, and of all
+  Seen only;                         // of a lane's one sequence: its length is read once
   __device__ Cut(const AttentionArgs& a) : run((a.sequences + 63) / 64) {
     const int first = (int)(threadIdx.x & 63) * run;
     double total = 0.0;  // exact: below 2^41
-    for (int i = 0; i < run; ++i) {
-      if (first + i < a.sequences) total += (double)Seen(a, first + i).seen;
+    if (run == 1) {
+      if (first < a.sequences) only = Seen(a, first);
+      total = (double)only.seen;
+    } else {
+      for (int i = 0; i < run; ++i) {
+        if (first + i < a.sequences) total += (double)Seen(a, first + i).seen;
+      }
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
@@ -161,7 +173,9 @@ struct Cut {
     before = sum - mine;
     all = __builtin_amdgcn_readlane(sum, 63);
   }
+  // Of one of the lane's sequences.
   __device__ int parts_of(const AttentionArgs& a, int sequence) const {
+    if (run == 1) return (only.seen + each - 1) / each;  // the lane's; 0 behind the last sequence
     return sequence < a.sequences ? (Seen(a, sequence).seen + each - 1) / each : 0;
   }
   // First part and number of parts of each sequence, for the launch that joins them.
@@ -188,11 +202,14 @@ struct Part {
   bool none = false;
   __device__ Part(const AttentionArgs& a, int id) {
     const int units = a.kv_heads * a.head_tiles;
-    int part = 0, each = INT32_MAX;
+    int part = 0, each = INT32_MAX, seen, lo;
     if (a.parts == 0) {
       id = xcd_contiguous(id, a.sequences * units);
       sequence = index = id / units;
       unit = id - index * units;
+      const Seen s(a, sequence);
+      seen = __builtin_amdgcn_readfirstlane(s.seen);
+      lo = __builtin_amdgcn_readfirstlane(s.lo);
     } else {
       const Cut cut(a);
       each = cut.each;
@@ -212,10 +229,11 @@ struct Part {
       const int lane = __builtin_ctzll(owner);
       sequence = __builtin_amdgcn_readlane(found, lane);
       part = __builtin_amdgcn_readlane(in, lane);
+      const Seen s = cut.run == 1 ? cut.only : Seen(a, sequence);
+      seen = __builtin_amdgcn_readlane(s.seen, lane);
+      lo = __builtin_amdgcn_readlane(s.lo, lane);
+      count = (seen + each - 1) / each;
     }
-    const Seen s(a, sequence);
-    const int seen = __builtin_amdgcn_readfirstlane(s.seen), lo = __builtin_amdgcn_readfirstlane(s.lo);
-    if (a.parts > 0) count = (seen + each - 1) / each;
     begin = lo + part * (a.parts > 0 ? each : 0);
     end = seen - part * (a.parts > 0 ? each : 0) <= each ? lo + seen : begin + each;
   }
@@ -263,7 +281,7 @@ __device__ inline void store4(const f32x4& v, char* p) {
 }
 
 // 16 bytes per lane from p to LDS at the named place + 16 x lane (see lds_place), as data that is
-// read once: 207 us in place of 236 for the 64 ragged sequences below.
+// read once: 13 % less time for 64 ragged sequences of up to 8192 positions.
 __device__ inline void load_to_place_from(const char* p) {
   asm volatile("global_load_lds_dwordx4 %0, off nt" ::"v"(p) : "memory");
 }
@@ -279,14 +297,18 @@ __device__ inline u32x2 codes_at(LdsPtr from, int f, int g, int col) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(reinterpret_cast<Lds2>(p)));
 }
 
-template <class T, class S, int DIM>
-__global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
+// WAVES: those of a workgroup, which share its positions and meet in LDS; more than one only where each sequence is
+// one part.
+template <class T, class S, int DIM, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 1) void paged_attention(AttentionArgs a) {
   using Sh = Shape<T, S, DIM>;
   constexpr int kTiles = Sh::kTiles, kStep = Sh::kStep, kOfLane = Sh::kOfLane, kFrags = S::kFragments;
   constexpr int kRow = Sh::kRow, kAll = 2 * Sh::kLoads;
   constexpr int kDepth = Sh::kDepth;
-  __shared__ __attribute__((aligned(1024))) char lds[kDepth * Sh::kSlot];
-  __shared__ int found[kFound];
+  constexpr int kOut = DIM / 16;
+  static_assert(16 * DIM * 4 <= kDepth * Sh::kSlot);
+  __shared__ __attribute__((aligned(1024))) char rings[WAVES][kDepth * Sh::kSlot];
+  __shared__ __attribute__((aligned(16))) int founds[WAVES][kFound];
 
   const Part span(a, (int)blockIdx.x);
   if (span.none) return;
@@ -294,8 +316,25 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
   const int kv = unit / a.head_tiles, group = a.heads / a.kv_heads;
   const int head0 = unit % a.head_tiles * kHeads, heads = group - head0 < kHeads ? group - head0 : kHeads;
 
-  const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
+  const int wave = wave_of<WAVES>(), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  char* const lds = rings[wave];
+  int* const found = founds[wave];
   const int row_bytes = a.dim * S::kBytes;
+
+  if (span.begin == span.end) {  // of a sequence that is one part; others have none then
+    const int64_t first = (int64_t)sequence * a.heads + kv * group + head0;
+    for (int e = (int)threadIdx.x * 4; e < heads * a.dim; e += 256 * WAVES) {
+      store4<typename T::Codec>((f32x4){0.0f, 0.0f, 0.0f, 0.0f}, a.out + (first * a.dim + e) * T::kBytes);
+    }
+    if ((int)threadIdx.x < heads && a.lse != nullptr) a.lse[first + threadIdx.x] = -__builtin_inff();
+    return;
+  }
+  int begin = span.begin, end = span.end;
+  if constexpr (WAVES > 1) {
+    const int each = ((end - begin + WAVES - 1) / WAVES + kStep - 1) / kStep * kStep;
+    begin += wave * each;
+    end = end - begin < each ? end : begin + each;  // no more than begin: nothing for this wave
+  }
 
   // The columns' queries: of each chunk of a row the elements that this lane has.
   u32x4 q[kOfLane][kFrags];
@@ -313,13 +352,6 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
     }
   }
 
-  // They are here before the loop: a wait of the compiler's inside it would be one for the steps on their way too.
-#pragma unroll
-  for (int s = 0; s < kOfLane; ++s) {
-#pragma unroll
-    for (int f = 0; f < kFrags; ++f) asm volatile("" : "+v"(q[s][f]));
-  }
-
   // Slots of the positions from `first` on, kFound of them; -1 for none.
   const int64_t* table = a.table + (int64_t)sequence * a.table_width;
   auto find = [&](int first, auto each) __attribute__((always_inline)) {
@@ -328,7 +360,7 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
     int in_page[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int t = first + i * 64 + lane, last = span.end - 1;
+      const int t = first + i * 64 + lane, last = end - 1;
       const uint32_t u = (uint32_t)(t < last ? t : last);
       const uint32_t at = (uint32_t)(((uint64_t)u * a.page_magic) >> a.page_shift);
       page[i] = table[at];
@@ -336,11 +368,18 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const bool there = first + i * 64 + lane < span.end && page[i] >= 0 && page[i] < a.pages;
+      const bool there = first + i * 64 + lane < end && page[i] >= 0 && page[i] < a.pages;
       found[i * 64 + lane] = there ? (int)page[i] * a.page + in_page[i] : -1;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+  };
+  auto look = [&](int first) __attribute__((always_inline)) {
+    if (end - first <= 64) {
+      find(first, IntC<1>{});
+    } else {
+      find(first, IntC<kFound / 64>{});
+    }
   };
   // The lane's row and chunk of a load instruction's kRows rows.
   const int load_row = lane / Sh::kChunks, load_chunk = lane % Sh::kChunks;
@@ -348,14 +387,8 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
   const char *const keys = a.keys + (int64_t)kv * row_bytes, *const values = a.values + (int64_t)kv * row_bytes;
   // Asks for a step of keys and values; which of its positions there are.
   auto ask = [&](int first, LdsPtr to) __attribute__((always_inline)) {
-    const int at = first - span.begin;
-    if (at % kFound == 0) {
-      if (span.end - first <= 64) {
-        find(first, IntC<1>{});
-      } else {
-        find(first, IntC<kFound / 64>{});
-      }
-    }
+    const int at = first - begin;
+    if (at > 0 && at % kFound == 0) look(first);
     const int mine = found[at % kFound + (lane & (kStep - 1))];
 #pragma unroll
     for (int i = 0; i < Sh::kLoads; ++i) {
@@ -374,7 +407,6 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
     return (uint32_t)__ballot(mine >= 0);
   };
 
-  constexpr int kOut = DIM / 16;
   f32x4 out[kOut] = {};
   // P is taken by base: top - kLift, or 0 while there is none.
   float top = -__builtin_inff(), base = 0.0f, sum = 0.0f;
@@ -508,26 +540,35 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
   };
 
   const LdsPtr slots = (LdsPtr)lds;
-  const int begin = span.begin, end = span.end;
-  uint32_t seen[kDepth] = {};
+  if (WAVES == 1 || begin < end) {
+    uint32_t seen[kDepth] = {};
+    look(begin);
+    // The queries are here, as the slots are: a wait of the compiler's inside the loop would be one for the steps on
+    // their way too.
 #pragma unroll
-  for (int d = 0; d < kDepth; ++d) {
-    if (begin + d * kStep < end) seen[d] = ask(begin + d * kStep, slots + d * Sh::kSlot);
-  }
-  for (int first = begin; first < end; first += kDepth * kStep) {
+    for (int s = 0; s < kOfLane; ++s) {
+#pragma unroll
+      for (int f = 0; f < kFrags; ++f) asm volatile("" : "+v"(q[s][f]));
+    }
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
-      const int now = first + d * kStep;
-      if (now < end) {
-        if (now + (kDepth - 1) * kStep < end) {
-          loads_landed<(kDepth - 1) * kAll>();
-        } else {
-          loads_landed();
-        }
-        step(slots + d * Sh::kSlot, seen[d]);
-        if (now + kDepth * kStep < end) {
-          lds_read();
-          seen[d] = ask(now + kDepth * kStep, slots + d * Sh::kSlot);
+      if (begin + d * kStep < end) seen[d] = ask(begin + d * kStep, slots + d * Sh::kSlot);
+    }
+    for (int first = begin; first < end; first += kDepth * kStep) {
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) {
+        const int now = first + d * kStep;
+        if (now < end) {
+          if (now + (kDepth - 1) * kStep < end) {
+            loads_landed<(kDepth - 1) * kAll>();
+          } else {
+            loads_landed();
+          }
+          step(slots + d * Sh::kSlot, seen[d]);
+          if (now + kDepth * kStep < end) {
+            lds_read();
+            seen[d] = ask(now + kDepth * kStep, slots + d * Sh::kSlot);
+          }
         }
       }
     }
@@ -536,6 +577,43 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
   sum += __shfl_xor(sum, 32);
   top -= T::kLift;  // the sums' power of two from here on
 
+  if constexpr (WAVES > 1) {
+    // As join_parts, of the waves.
+    float* const sums = reinterpret_cast<float*>(lds);
+    if (col < heads) {
+#pragma unroll
+      for (int f = 0; f < kOut; ++f) *reinterpret_cast<f32x4*>(sums + col * DIM + 16 * f + 4 * g) = out[f];
+    }
+    if (g == 0) *reinterpret_cast<f32x2*>(found + 2 * col) = (f32x2){top, sum};
+    __syncthreads();
+    const int quads = a.dim / 4;
+    for (int i = threadIdx.x; i < heads * quads; i += 64 * WAVES) {
+      const int h = i / quads, quad = i - h * quads;
+      f32x2 stats[WAVES];
+      float all_top = -__builtin_inff(), total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        stats[w] = *reinterpret_cast<const f32x2*>(founds[w] + 2 * h);
+        all_top = __builtin_fmaxf(all_top, stats[w][0]);
+      }
+      const float all_base = all_top == -__builtin_inff() ? 0.0f : all_top;
+      f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float p = __builtin_amdgcn_exp2f(stats[w][0] - all_base);
+        o += p * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(rings[w]) + h * DIM + 4 * quad);
+        total += p * stats[w][1];
+      }
+      const int64_t head = (int64_t)sequence * a.heads + kv * group + head0 + h;
+      const float inverse = total == 0.0f ? 0.0f : a.value_scale / total;
+      o = total == 0.0f ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : o * inverse;
+      store4<typename T::Codec>(o, a.out + (head * a.dim + 4 * quad) * T::kBytes);
+      if (quad == 0 && a.lse != nullptr) {
+        a.lse[head] = total == 0.0f ? -__builtin_inff() : (all_top + __builtin_log2f(total)) * kLn2;
+      }
+    }
+    return;
+  }
   if (col >= heads) return;
   const int in_sequence = kv * group + head0 + col;
   const int64_t head = (int64_t)sequence * a.heads + in_sequence;
@@ -565,7 +643,6 @@ __global__ __launch_bounds__(64, 1) void paged_attention(AttentionArgs a) {
   }
 }
 
-constexpr int kMaxParts = 1024;  // of all sequences, or twice as many as there are of them
 constexpr int64_t kMaxPositions = int64_t(1) << 30;  // of a sequence: a step past the last is still an int
 constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
 constexpr int kMaxCut = 2048;  // sequences: beyond it each is one part, so that nobody reads so many lengths
@@ -638,30 +715,73 @@ int64_t bytes_of(int32_t dtype) { return dtype == kF32 ? 4 : dtype == kF16 || dt
 
 int head_tiles_of(int64_t heads, int64_t kv_heads) { return (int)((heads / kv_heads + kHeads - 1) / kHeads); }
 
-// Parts of all sequences together, or 0 where each is one: as many as fill the LDS of the
-// 256 CUs, and eight times the sequences, for lengths that differ.
-int parts_of(int64_t sequences, int64_t units, int64_t positions, int64_t dim, int64_t cache_bytes) {
+// Bytes of LDS of a step's keys and values.
+int64_t step_bytes(int64_t dim, int64_t cache_bytes) {
+  return (cache_bytes == 4 ? 16 : 32) * (dim <= 64 ? 64 : dim <= 128 ? 128 : 256) * cache_bytes * 2;
+}
+
+// Parts of all sequences together, at most, or 0 where each is one. Few sequences: as many as fill the LDS of the 256
+// CUs, all of one length. More of them end in parts that are shorter and leave CUs to wait, so then there are several
+// for each place; each costs about what kPartCost positions do, and the sum of both is least for a square root.
+// bf16, 8 heads of 128, ragged (a part for each place, this, 8 parts a sequence, us): 64 sequences of up to 1024
+// positions 33, 35, 37, of 8192 192, 191, 193; 128 of 512 37, 37, 51, of 4096 202, 192, 205; 32 of 4096 56, 55, 57.
+constexpr double kPartCost = 150;
+int64_t parts_of(int64_t sequences, int64_t units, int64_t positions, int64_t dim, int64_t cache_bytes) {
   if (positions <= kMinPart || sequences > kMaxCut) return 0;
-  const int64_t padded = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-  const int64_t two = (cache_bytes == 4 ? 16 : 32) * padded * cache_bytes * 2 * 2;
+  const int64_t two = 2 * step_bytes(dim, cache_bytes);
   const int64_t slots = 256 * (160 * 1024 / ((two > kRing ? two : kRing) + kFound * 4));
-  int64_t parts = (slots + units - 1) / units;
-  parts = parts > 8 * sequences ? parts : 8 * sequences;
-  const int64_t limit = 2 * sequences > kMaxParts ? 2 * sequences : kMaxParts;
-  parts = parts < limit ? parts : limit;
+  const int64_t at_once = (slots + units - 1) / units;
+  int64_t parts = at_once;
+  if (4 * sequences > at_once) {
+    const double half = 0.5 * (double)(sequences * positions);  // lengths differ
+    const int64_t more = (int64_t)__builtin_sqrt(half * (double)at_once / kPartCost);
+    parts = sequences + (more < 8 * at_once ? more : 8 * at_once);
+    parts = parts > at_once ? parts : at_once;
+    parts = parts > 2 * sequences ? parts : 2 * sequences;
+  }
   const int64_t most = sequences * ((positions + kMinPart - 1) / kMinPart) + sequences;  // of the shortest parts
   parts = parts < most ? parts : most;
-  return parts * units <= kMaxBlocks ? (int)parts : 0;  // so many heads fill the card by themselves
+  return parts * units <= kMaxBlocks ? parts : 0;  // so many heads fill the card by themselves
+}
+
+// Who takes a sequence of a key-value head: a wave, the waves of a workgroup, or parts of it are shared out. Without
+// parts there is no second launch, and no length but its own to read, but where one sequence is much longer than the
+// others its waves are waited for: a step costs a wave 1 us alone.
+// A wave, for steps that are few for the number of them (B workgroups). bf16, 8 heads of 128, ragged, up to so many
+// positions, us, a wave, waves and parts: B 8192: 64 42, 117, 231; 512 182, 228, 362. B 2048: 64 12, 30, 32; 512 53, 62,
+// 65; 1024 106, 99, 110. B 512: 64 6.6, 8.6, 9.9; 256 12.7, 12.3, 13.6; 512 20.9, 18.8, 20.9.
+// Waves, for contexts that they are through with soon; the more work there is beside it, the longer. Us, waves and
+// parts: B 8: 256 6.8, 9.6; 768 10.2, 11.2; 1024 12.4, 11.2. B 64: 512 9.0, 10.9; 1024 15.2, 12.3. B 256: 1024 17.1,
+// 20.0; 2048 30.9, 31.1. B 1024: 1024 55, 61; 2048 99, 103. B 2048: 2048 183, 198.
+enum Way { kWave, kWaves, kParts };
+Way way_of(int64_t blocks, int64_t seen, int64_t dim, int64_t cache_bytes) {
+  const int64_t bytes = step_bytes(dim, cache_bytes), each = cache_bytes == 4 ? 16 : 32;
+  const int64_t steps = (seen + each - 1) / each;
+  if (steps <= 2 || steps <= blocks / 128) return kWave;
+  const int64_t waves = 2 * bytes > kRing ? 2 : 4;
+  const int64_t soon = blocks < 128 ? 6 : blocks < 1024 ? 8 : 16;  // of a wave, of 16 KB or less
+  return steps <= waves * (bytes > kRing / 2 ? soon / 2 : soon) ? kWaves : kParts;
+}
+
+template <class T, class S, int DIM>
+void run_waves(const AttentionArgs& a, int64_t blocks, bool whole, hipStream_t st) {
+  using Sh = Shape<T, S, DIM>;
+  constexpr int kWaves = Sh::kDepth * Sh::kSlot > kRing ? 2 : 4;  // rings that fit a CU's LDS
+  if (whole) {
+    paged_attention<T, S, DIM, kWaves><<<(unsigned)blocks, 64 * kWaves, 0, st>>>(a);
+  } else {
+    paged_attention<T, S, DIM, 1><<<(unsigned)blocks, 64, 0, st>>>(a);
+  }
 }
 
 template <class T, class S>
-int32_t run_dim(const AttentionArgs& a, int64_t blocks, hipStream_t st) {
+int32_t run_dim(const AttentionArgs& a, int64_t blocks, bool whole, hipStream_t st) {
   if (a.dim <= 64) {
-    paged_attention<T, S, 64><<<(unsigned)blocks, 64, 0, st>>>(a);
+    run_waves<T, S, 64>(a, blocks, whole, st);
   } else if (a.dim <= 128) {
-    paged_attention<T, S, 128><<<(unsigned)blocks, 64, 0, st>>>(a);
+    run_waves<T, S, 128>(a, blocks, whole, st);
   } else {
-    paged_attention<T, S, 256><<<(unsigned)blocks, 64, 0, st>>>(a);
+    run_waves<T, S, 256>(a, blocks, whole, st);
   }
   int32_t status = launch_status();
   if (status == 0 && a.parts > 0) {
@@ -678,10 +798,10 @@ int32_t run_dim(const AttentionArgs& a, int64_t blocks, hipStream_t st) {
 }
 
 template <class T>
-int32_t run_cache(const AttentionArgs& a, int64_t blocks, int32_t cache_dtype, hipStream_t st) {
-  if (cache_dtype == kF8E4M3) return run_dim<T, FromCodes<T, kF8E4M3>>(a, blocks, st);
-  if (cache_dtype == kF8E5M2) return run_dim<T, FromCodes<T, kF8E5M2>>(a, blocks, st);
-  return run_dim<T, AsIs<T>>(a, blocks, st);
+int32_t run_cache(const AttentionArgs& a, int64_t blocks, bool whole, int32_t cache_dtype, hipStream_t st) {
+  if (cache_dtype == kF8E4M3) return run_dim<T, FromCodes<T, kF8E4M3>>(a, blocks, whole, st);
+  if (cache_dtype == kF8E5M2) return run_dim<T, FromCodes<T, kF8E5M2>>(a, blocks, whole, st);
+  return run_dim<T, AsIs<T>>(a, blocks, whole, st);
 }
 
 bool attention_sizes_ok(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, int64_t page,
@@ -740,7 +860,11 @@ extern "C" int32_t launch_paged_attention_fwd(const void* q, const void* key_cac
   a.window = window > 0 && window < INT32_MAX ? (int)window : 0;
   a.head_tiles = head_tiles_of(n_q_heads, n_kv_heads);
   const int64_t units = n_kv_heads * a.head_tiles;
-  a.parts = parts_of(sequences, units, page_size * table_width, head_dim, bytes_of(cache_dtype));
+  const int64_t positions = page_size * table_width, seen = a.window > 0 && a.window < positions ? a.window : positions;
+  a.parts = (int)parts_of(sequences, units, positions, head_dim, bytes_of(cache_dtype));
+  const Way way = way_of(sequences * units, seen, head_dim, bytes_of(cache_dtype));
+  if (way != kParts) a.parts = 0;
+  const bool whole = way != kWave && a.parts == 0;
   if (a.parts > 0 && (workspace == nullptr || !host_aligned(workspace, 16))) return (int32_t)hipErrorInvalidValue;
   // t / page for t < 2^31: t * magic >> shift, magic = floor(2^(31 + bits) / page) + 1 with
   // 2^bits >= page. What magic is too large by, at most 1, adds less than 2^-bits <= 1 / page.
@@ -753,8 +877,8 @@ extern "C" int32_t launch_paged_attention_fwd(const void* q, const void* key_cac
   const int64_t blocks = (a.parts > 0 ? a.parts : sequences) * units;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case kF32: return run_cache<F32>(a, blocks, cache_dtype, st);
-    case kF16: return run_cache<F16>(a, blocks, cache_dtype, st);
-    default: return run_cache<Bf16>(a, blocks, cache_dtype, st);
+    case kF32: return run_cache<F32>(a, blocks, whole, cache_dtype, st);
+    case kF16: return run_cache<F16>(a, blocks, whole, cache_dtype, st);
+    default: return run_cache<Bf16>(a, blocks, whole, cache_dtype, st);
   }
 }

@@ -270,3 +270,77 @@ def test_most_heads():
     out, lse = K.paged_attention(q, keys, values, table.cuda(), lengths.cuda(), return_lse=True)
     some = torch.tensor([0, 1, 48, 1000, b - 1])
     _check(q[some].cpu(), keys.cpu(), values.cpu(), table[some], lengths[some], got=(out[some], lse[some]))
+
+
+# ---------------------------------------------------------------------------
+# Who takes a sequence - a wave, a workgroup's waves, or parts of it are shared out - is chosen by how many positions
+# the table has room for: the same sequences with wider tables.
+# ---------------------------------------------------------------------------
+
+def _wide(table, pages):
+    return torch.cat([table, torch.full((table.shape[0], pages), -1)], 1)
+
+
+@pytest.mark.parametrize("lengths", [[0, 1, 17, 130, 333], [2500, 31, 0, 1030]], ids=["short", "long"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("heads,kv,dim,cache", [
+    (8, 8, 64, None), (32, 8, 128, None), (12, 4, 80, None), (14, 2, 192, None), (8, 2, 256, None), (40, 2, 48, None),
+    (8, 2, 128, torch.float8_e4m3fn), (12, 4, 80, torch.float8_e5m2), (16, 1, 256, torch.float8_e4m3fn),
+    (4, 2, 16, torch.float8_e5m2)])
+def test_ways(heads, kv, dim, cache, dtype, lengths):
+    q, keys, values, table, lengths = _case(lengths, heads, kv, dim, 16, dtype, cache, seed=heads + dim)
+    kw = {} if cache is None else {"key_scale": 0.31, "value_scale": 1.7}
+    for pages in (0, 1, 30, 1000):
+        _check(q, keys, values, _wide(table, pages), lengths, **kw)
+
+
+@pytest.mark.parametrize("page", [1, 3, 13, 100, 256])
+@pytest.mark.parametrize("window", [0, 5, 129, 900, 1500])
+def test_windows_and_pages_of_long_sequences(page, window):
+    q, keys, values, table, lengths = _case([1300, 0, 2100, 1, 899, 900, 901], 4, 2, 64, page, torch.float16, seed=page)
+    table[2, 700 // page] = -1
+    _check(q, keys, values, table, lengths, window=window)
+    _check(q, keys, values, _wide(table, 4096 // page), lengths, window=window)
+
+
+@pytest.mark.parametrize("pages", [0, 1000])
+def test_what_is_not_seen_of_any_way(pages):
+    q, keys, values, table, lengths = _case([37, 1200, 16], 8, 2, 128, 16, torch.bfloat16, seed=61)
+    args = q.cuda(), keys.cuda(), values.cuda(), _wide(table, pages).cuda(), lengths.cuda()
+    for window in (0, 50):
+        want = K.paged_attention(*args, window=window)
+        seen = torch.zeros(keys.shape[:2], dtype=torch.bool)
+        for b in range(3):
+            t = torch.arange(max(0, int(lengths[b]) - window) if window else 0, int(lengths[b]))
+            seen[table[b, t // 16], t % 16] = True
+        for bad in (float("nan"), float("inf"), -float("inf"), torch.finfo(torch.bfloat16).min):
+            for target in (args[1], args[2]):
+                target[~seen.cuda()] = bad
+            assert torch.equal(K.paged_attention(*args, window=window), want), (bad, window)
+        args = q.cuda(), keys.cuda(), values.cuda(), *args[3:]
+
+
+@pytest.mark.parametrize("count,most", [(300, 40), (300, 200), (300, 700), (70, 200), (70, 1500), (2100, 300)])
+def test_batches(count, most):
+    g = torch.Generator().manual_seed(count + most)
+    lengths = torch.randint(0, most + 1, (count,), generator=g).tolist()
+    lengths[count // 2] = most
+    _check(*_case(lengths, 4, 4, 32, 16, torch.bfloat16, seed=62))
+
+
+@pytest.mark.parametrize("pages", [0, 1000])
+def test_each_way_into_a_graph(pages):
+    """Replayed with other lengths and queries, eager calls between."""
+    q, keys, values, table, lengths = _case([400, 130, 0, 777], 8, 2, 128, 16, torch.bfloat16, seed=63)
+    args = q.cuda(), keys.cuda(), values.cuda(), _wide(table, pages).cuda(), lengths.cuda()
+    K.paged_attention(*args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = K.paged_attention(*args)
+    for i in range(4):
+        args[4].copy_(torch.tensor([400 - 99 * i, i, 130 * i, 777 // (i + 1)]))
+        args[0].copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, K.paged_attention(*args)), i
