@@ -186,11 +186,14 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product(BlockArgs a) {
   constexpr int kAtQ = P::kLds, kAtS = kAtQ + Q::kLds, kSlot = kAtS + S::kLds, kLds = 2 * kSlot;
   constexpr int kAll = P::kLoads + Q::kLoads + 1;
   static_assert(FQ * 16 <= 128 && 128 % (FQ * 16) == 0);  // a wave's columns share a scale
-  // Columns that are multiplied while the others are read. Then the waves meet, once a step: this slot is free, and
-  // the next one has landed. The loads of the step after that go out between the products of the rest: at once they
-  // would hold each other up, with the matrix cores idle. 8192 rows, 14336 x 4096, us: 420; at once 460, with a meeting
-  // of its own for each of the two 445.
-  constexpr int kFirst = FQ / 2;
+  // A wave has kAhead columns' codes in registers: behind the products of column j it reads column j + kAhead, of this
+  // step or the next one, and behind those of the last one the next step's rows, so that a step begins with what it
+  // needs. Behind the products of column kLast the waves meet, once a step: this slot has been read, and the next one
+  // has landed. The loads of the step after that go out between the products that are left: at once they would hold
+  // each other up, with the matrix cores idle. 8192 rows, 14336 x 4096, us: 419, and with 16384 products a sum 1543; a
+  // step's first codes read when it begins 426 and 1600, loads at once 460, a second meeting 445. Two columns ahead in
+  // place of four 436 and 1600.
+  constexpr int kAhead = FQ == 8 ? 4 : 2, kLast = FQ - kAhead;
   __shared__ __attribute__((aligned(1024))) char lds[kLds];
   __shared__ typename RowTiles<BP, NW * 64>::Shared shared;
 
@@ -245,61 +248,72 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product(BlockArgs a) {
   advance();
   loads_landed<kAll>();
   meet();
+  u32x4 x[FP][2], w[kAhead][2];
+  BlockFragment<FX, EXACT> wide[FP];  // EXACT: x, once a step
+  float scale[FP], next[FP], of_cols = 0.0f;
+  f32x4 part[FP];
+  auto read_x = [&](int i, int slot) __attribute__((always_inline)) {
+    x[i][0] = p_lane.fragment(i, 0, slot);
+    x[i][1] = p_lane.fragment(i, 1, slot);
+    next[i] = S::row(slots + slot + kAtS, p0 + 16 * i + (lane & 15));
+  };
+  auto read_w = [&](int j, int slot) __attribute__((always_inline)) {
+    w[j % kAhead][0] = q_lane.fragment(j, 0, slot);
+    w[j % kAhead][1] = q_lane.fragment(j, 1, slot);
+  };
+  if (live) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) read_w(j, 0);
+#pragma unroll
+    for (int i = 0; i < FP; ++i) {
+      read_x(i, 0);
+      scale[i] = 0.0f;
+      part[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    of_cols = S::cols(slots + kAtS, q0);
+  }
   for (int t = 0; t < a.blocks; ++t) {
-    const int slot = (t & 1) * kSlot;
+    const int slot = (t & 1) * kSlot, other = kSlot - slot;
     const LdsPtr now = slots + slot;
     if (live) {
-      BlockFragment<FX, EXACT> x[FP];
-      BlockFragment<FW, EXACT> w[FQ];
-      float scale[FP];
-      auto columns = [&](int j) __attribute__((always_inline)) {
-        w[j] = BlockFragment<FW, EXACT>(q_lane.fragment(j, 0, slot), q_lane.fragment(j, 1, slot));
-      };
-      columns(0);
-#pragma unroll
-      for (int i = 0; i < FP; ++i) {
-        x[i] = BlockFragment<FX, EXACT>(p_lane.fragment(i, 0, slot), p_lane.fragment(i, 1, slot));
-      }
-      const float of_cols = S::cols(now + kAtS, q0);
-#pragma unroll
-      for (int i = 0; i < FP; ++i) scale[i] = S::row(now + kAtS, p0 + 16 * i + (lane & 15));
-      // Each product is added FP products later, when the matrix cores are done with it.
-      f32x4 part[FP];
 #pragma unroll
       for (int j = 0; j < FQ; ++j) {
-        if (j < kFirst) {
-          columns(2 * j + 1);
-          if (2 * j + 2 < FQ) columns(2 * j + 2);
-        }
-        if (j == kFirst) {
-          lds_read();
-          loads_landed();
-          meet();  // this slot has been read, and the next has landed
-        }
-        if (j == 1) {
-#pragma unroll
-          for (int i = 0; i < FP; ++i) scale[i] *= of_cols;
-        }
+        const BlockFragment<FW, EXACT> column(w[j % kAhead][0], w[j % kAhead][1]);
 #pragma unroll
         for (int i = 0; i < FP; ++i) {
-          if (j > 0) add_scaled(acc[i][j - 1], part[i], scale[i]);
-          part[i] = block_mma<FX, FW, EXACT>(w[j], x[i]);
-          if (j >= kFirst) {
-            constexpr int kSpread = (FQ - kFirst) * FP;
-            const int n = (j - kFirst) * FP + i;
+          // Each product is added FP products later, when the matrix cores are done with it.
+          add_scaled(acc[i][j == 0 ? FQ - 1 : j - 1], part[i], scale[i]);
+          if (j == 0) {
+            scale[i] = next[i] * of_cols;
+            if (EXACT) wide[i] = BlockFragment<FX, EXACT>(x[i][0], x[i][1]);
+          }
+          part[i] = block_mma<FX, FW, EXACT>(column, EXACT ? wide[i] : BlockFragment<FX, EXACT>(x[i][0], x[i][1]));
+          if (j == FQ - 1) read_x(i, other);
+          if (j > kLast) {
+            constexpr int kSpread = (FQ - 1 - kLast) * FP;
+            const int n = (j - kLast - 1) * FP + i;
             ask(now, n * kAll / kSpread, (n + 1) * kAll / kSpread);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
+        if (j == kLast) {
+          lds_read();
+          loads_landed();
+          meet();
+        }
+        read_w((j + kAhead) % FQ, j < kLast ? slot : other);
+        if (j == FQ - 1) of_cols = S::cols(slots + other + kAtS, q0);
       }
-#pragma unroll
-      for (int i = 0; i < FP; ++i) add_scaled(acc[i][FQ - 1], part[i], scale[i]);
     } else {
       loads_landed();
       meet();
       ask(now, 0, kAll);
     }
     advance();
+  }
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < FP; ++i) add_scaled(acc[i][FQ - 1], part[i], scale[i]);
   }
   loads_landed();
   meet();  // nobody reads the slots any more, and nothing is on its way to them
