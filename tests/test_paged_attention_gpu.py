@@ -344,3 +344,15 @@ def test_each_way_into_a_graph(pages):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, K.paged_attention(*args)), i
+
+
+@pytest.mark.parametrize("most", [700, 3000])
+def test_more_sequences_than_are_cut(most):
+    g = torch.Generator().manual_seed(64)
+    q = torch.randn((2100, 2, 16), generator=g).half()
+    keys, values = (torch.randn((200, 16, 1, 16), generator=g).half() for _ in range(2))
+    table = torch.randint(0, 200, (2100, -(-most // 16)), generator=g)
+    lengths = torch.randint(0, 100, (2100,), generator=g)
+    lengths[::70] = torch.randint(0, most + 1, (30,), generator=g)
+    lengths[[5, 2099]] = most
+    _check(q, keys, values, table, lengths)
