@@ -53,6 +53,7 @@ struct AttentionArgs {
   uint32_t page_magic;
   int page_shift;
   float score_scale, value_scale;  // score_scale: with log2(e)
+  float part_cost;                 // kPartCost for each of the places, or 0: see parts_of
 };
 
 using i32x2 = int __attribute__((ext_vector_type(2)));
@@ -159,7 +160,9 @@ struct Cut {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
     // Each sequence has a last part that may be short, so that there are no more than a.parts in all.
-    const int wanted = (int)__builtin_ceil(total / (double)(a.parts - a.sequences));
+    // The host has allowed for as many as the table has room for; what the lengths call for may be fewer.
+    const double even = total / (double)(a.parts - a.sequences), worth = __builtin_sqrt(total * a.part_cost);
+    const int wanted = (int)__builtin_ceil(even > worth ? even : worth);
     each = __builtin_amdgcn_readfirstlane((wanted + kMinPart - 1) / kMinPart * kMinPart);
     each = each < kMinPart ? kMinPart : each;
     mine = 0;
@@ -722,21 +725,28 @@ int64_t step_bytes(int64_t dim, int64_t cache_bytes) {
 
 // Parts of all sequences together, at most, or 0 where each is one. Few sequences: as many as fill the LDS of the 256
 // CUs, all of one length. More of them end in parts that are shorter and leave CUs to wait, so then there are several
-// for each place; each costs about what kPartCost positions do, and the sum of both is least for a square root.
-// bf16, 8 heads of 128, ragged (a part for each place, this, 8 parts a sequence, us): 64 sequences of up to 1024
-// positions 33, 35, 37, of 8192 192, 191, 193; 128 of 512 37, 37, 51, of 4096 202, 192, 205; 32 of 4096 56, 55, 57.
+// for each place; each costs about what kPartCost positions do, and the sum of both is least for a square root. The
+// host takes half of the positions that the table has room for, the workgroups what there are: then many of the grid's
+// find nothing to do, so it is limited. bf16, 8 heads of 128, ragged, us, this and 8 parts a sequence: 64 of up to 8192
+// 191, 193; 128 of up to 4096 192, 205; 32 of up to 4096 55, 57; 64 of up to 1000 in tables for 131072 32, 36; 128 in
+// tables for 32768 57, 67; 64 of up to 32768 729, 712.
 constexpr double kPartCost = 150;
-int64_t parts_of(int64_t sequences, int64_t units, int64_t positions, int64_t dim, int64_t cache_bytes) {
-  if (positions <= kMinPart || sequences > kMaxCut) return 0;
+// Workgroups of a key-value head that fit the card.
+int64_t places_of(int64_t units, int64_t dim, int64_t cache_bytes) {
   const int64_t two = 2 * step_bytes(dim, cache_bytes);
   const int64_t slots = 256 * (160 * 1024 / ((two > kRing ? two : kRing) + kFound * 4));
-  const int64_t at_once = (slots + units - 1) / units;
-  int64_t parts = at_once;
-  if (4 * sequences > at_once) {
+  return (slots + units - 1) / units;
+}
+bool few(int64_t sequences, int64_t places) { return 4 * sequences <= places; }
+int64_t parts_of(int64_t sequences, int64_t units, int64_t positions, int64_t dim, int64_t cache_bytes) {
+  if (positions <= kMinPart || sequences > kMaxCut) return 0;
+  const int64_t places = places_of(units, dim, cache_bytes);
+  int64_t parts = places;
+  if (!few(sequences, places)) {
     const double half = 0.5 * (double)(sequences * positions);  // lengths differ
-    const int64_t more = (int64_t)__builtin_sqrt(half * (double)at_once / kPartCost);
-    parts = sequences + (more < 8 * at_once ? more : 8 * at_once);
-    parts = parts > at_once ? parts : at_once;
+    const int64_t more = (int64_t)__builtin_sqrt(half * (double)places / kPartCost);
+    parts = sequences + (more < 4 * places ? more : 4 * places);
+    parts = parts > places ? parts : places;
     parts = parts > 2 * sequences ? parts : 2 * sequences;
   }
   const int64_t most = sequences * ((positions + kMinPart - 1) / kMinPart) + sequences;  // of the shortest parts
@@ -864,6 +874,8 @@ extern "C" int32_t launch_paged_attention_fwd(const void* q, const void* key_cac
   a.parts = (int)parts_of(sequences, units, positions, head_dim, bytes_of(cache_dtype));
   const Way way = way_of(sequences * units, seen, head_dim, bytes_of(cache_dtype));
   if (way != kParts) a.parts = 0;
+  const int64_t places = places_of(units, head_dim, bytes_of(cache_dtype));
+  a.part_cost = few(sequences, places) ? 0.0f : (float)(kPartCost / (double)places);
   const bool whole = way != kWave && a.parts == 0;
   if (a.parts > 0 && (workspace == nullptr || !host_aligned(workspace, 16))) return (int32_t)hipErrorInvalidValue;
   // t / page for t < 2^31: t * magic >> shift, magic = floor(2^(31 + bits) / page) + 1 with
