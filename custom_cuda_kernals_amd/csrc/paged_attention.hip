@@ -35,6 +35,7 @@ constexpr int kHeads = 16;    // query heads of a workgroup, at most
 constexpr int kMinPart = 32;  // positions of a part, at least: a step
 constexpr int kFound = 512;   // positions whose slots are looked up at a time
 constexpr int kRing = 32768;  // bytes of LDS for the steps of a wave: more only if two steps need it
+constexpr int kMaxCut = 2048;  // sequences: beyond it each is one part, so that nobody reads so many lengths
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Sums are scaled to a new maximum only where it is this much (a power of two) above the
 // one that they have.
@@ -126,12 +127,17 @@ struct FromCodes {
 struct Seen {
   int lo = 0, seen = 0;
   __device__ Seen() = default;
-  __device__ Seen(const AttentionArgs& a, int sequence) {
+  // Of n positions.
+  __device__ Seen(const AttentionArgs& a, int n) {
+    lo = a.window > 0 && n > a.window ? n - a.window : 0;
+    seen = n - lo;
+  }
+  __device__ static int in_table(const AttentionArgs& a, int64_t n) {
     const int64_t most = (int64_t)a.table_width * a.page;
-    int64_t n = a.lengths[sequence];
-    n = n < 0 ? 0 : n > most ? most : n;
-    lo = a.window > 0 && n > a.window ? (int)n - a.window : 0;
-    seen = (int)n - lo;
+    return (int)(n < 0 ? 0 : n > most ? most : n);
+  }
+  __device__ static Seen of(const AttentionArgs& a, int sequence) {
+    return Seen(a, in_table(a, a.lengths[sequence]));
   }
 };
 
@@ -142,19 +148,32 @@ __device__ inline int* notes_of(const AttentionArgs& a) {
 
 // How the sequences are cut: into parts of `each` positions, numbered through all of them.
 // A lane has a run of sequences, and knows how many parts come before them. Every lane of
-// the wave calls.
+// the wave calls. The lengths of runs of more than one wait in `room`, in LDS.
 struct Cut {
   int each, run, mine, before, all;  // sequences of a run; parts of the lane's, before them, and of all
-  Seen only;                         // of a lane's one sequence: its length is read once
-  __device__ Cut(const AttentionArgs& a) : run((a.sequences + 63) / 64) {
+  Seen only;                         // of a lane's one sequence
+  const int* lengths;
+  __device__ Cut(const AttentionArgs& a, int* room) : run((a.sequences + 63) / 64), lengths(room) {
     const int first = (int)(threadIdx.x & 63) * run;
     double total = 0.0;  // exact: below 2^41
     if (run == 1) {
-      if (first < a.sequences) only = Seen(a, first);
+      if (first < a.sequences) only = Seen::of(a, first);
       total = (double)only.seen;
     } else {
+      constexpr int kAtOnce = 8;
+      for (int i = (int)(threadIdx.x & 63); i < a.sequences; i += 64 * kAtOnce) {
+        int64_t n[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) n[u] = a.lengths[i + 64 * u < a.sequences ? i + 64 * u : i];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          if (i + 64 * u < a.sequences) room[i + 64 * u] = Seen::in_table(a, n[u]);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
       for (int i = 0; i < run; ++i) {
-        if (first + i < a.sequences) total += (double)Seen(a, first + i).seen;
+        if (first + i < a.sequences) total += (double)Seen(a, lengths[first + i]).seen;
       }
     }
 #pragma unroll
@@ -179,7 +198,7 @@ struct Cut {
   // Of one of the lane's sequences.
   __device__ int parts_of(const AttentionArgs& a, int sequence) const {
     if (run == 1) return (only.seen + each - 1) / each;  // the lane's; 0 behind the last sequence
-    return sequence < a.sequences ? (Seen(a, sequence).seen + each - 1) / each : 0;
+    return sequence < a.sequences ? (Seen(a, lengths[sequence]).seen + each - 1) / each : 0;
   }
   // First part and number of parts of each sequence, for the launch that joins them.
   __device__ void note(const AttentionArgs& a) const {
@@ -203,18 +222,18 @@ struct Cut {
 struct Part {
   int index = 0, unit = 0, sequence = 0, begin = 0, end = 0, count = 1;
   bool none = false;
-  __device__ Part(const AttentionArgs& a, int id) {
+  __device__ Part(const AttentionArgs& a, int id, int* room) {
     const int units = a.kv_heads * a.head_tiles;
     int part = 0, each = INT32_MAX, seen, lo;
     if (a.parts == 0) {
       id = xcd_contiguous(id, a.sequences * units);
       sequence = index = id / units;
       unit = id - index * units;
-      const Seen s(a, sequence);
+      const Seen s = Seen::of(a, sequence);
       seen = __builtin_amdgcn_readfirstlane(s.seen);
       lo = __builtin_amdgcn_readfirstlane(s.lo);
     } else {
-      const Cut cut(a);
+      const Cut cut(a, room);
       each = cut.each;
       if (id == 0) cut.note(a);
       none = id >= cut.all * units;
@@ -232,7 +251,7 @@ struct Part {
       const int lane = __builtin_ctzll(owner);
       sequence = __builtin_amdgcn_readlane(found, lane);
       part = __builtin_amdgcn_readlane(in, lane);
-      const Seen s = cut.run == 1 ? cut.only : Seen(a, sequence);
+      const Seen s = cut.run == 1 ? cut.only : Seen(a, cut.lengths[sequence]);
       seen = __builtin_amdgcn_readlane(s.seen, lane);
       lo = __builtin_amdgcn_readlane(s.lo, lane);
       count = (seen + each - 1) / each;
@@ -309,11 +328,11 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_attention(AttentionArgs a
   constexpr int kRow = Sh::kRow, kAll = 2 * Sh::kLoads;
   constexpr int kDepth = Sh::kDepth;
   constexpr int kOut = DIM / 16;
-  static_assert(16 * DIM * 4 <= kDepth * Sh::kSlot);
+  static_assert(16 * DIM * 4 <= kDepth * Sh::kSlot && kMaxCut * 4 <= kDepth * Sh::kSlot);
   __shared__ __attribute__((aligned(1024))) char rings[WAVES][kDepth * Sh::kSlot];
   __shared__ __attribute__((aligned(16))) int founds[WAVES][kFound];
 
-  const Part span(a, (int)blockIdx.x);
+  const Part span(a, (int)blockIdx.x, reinterpret_cast<int*>(rings[0]));
   if (span.none) return;
   const int sequence = span.sequence, index = span.index, unit = span.unit;
   const int kv = unit / a.head_tiles, group = a.heads / a.kv_heads;
@@ -648,7 +667,6 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_attention(AttentionArgs a
 
 constexpr int64_t kMaxPositions = int64_t(1) << 30;  // of a sequence: a step past the last is still an int
 constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
-constexpr int kMaxCut = 2048;  // sequences: beyond it each is one part, so that nobody reads so many lengths
 
 // The sums of a sequence's parts, a head a workgroup. A thread has four elements of every
 // `lanes`-th part, and takes kAhead parts at a time.
