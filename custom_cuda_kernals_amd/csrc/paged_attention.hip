@@ -40,6 +40,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Sums are scaled to a new maximum only where it is this much (a power of two) above the
 // one that they have.
 constexpr float kSlack = 8.0f;
+// The power of two of P where sums passed float32's range: 2^30 values below 2^128 stay below 2^126.
+constexpr int kDown = -40;
 
 struct AttentionArgs {
   const char *q, *keys, *values;
@@ -63,7 +65,8 @@ using i32x2 = int __attribute__((ext_vector_type(2)));
 // row: 16 bytes.
 struct Bf16 {
   using Codec = CodecBF16;
-  static constexpr int kBytes = 2, kLift = 0;
+  static constexpr int kBytes = 2, kLift = 0, kLiftAgain = kDown;
+  static constexpr uint32_t kInfinity = 0x7f80u;
   __device__ static f32x4 mma(const u32x4& a, const u32x4& b, const f32x4& c) { return ElemBF16::mma(a, b, c, 0, 0); }
   __device__ static uint32_t pack(float lo, float hi) { return pack2_bf16(lo, hi); }
   __device__ static float low(uint32_t w) { return bf16_lo(w); }
@@ -72,7 +75,8 @@ struct Bf16 {
 struct F16 {
   using Codec = CodecF16;
   // P times 2^7: with kSlack 2^15 at most, and what a long tail of small ones has keeps its bits down to 2^-31.
-  static constexpr int kBytes = 2, kLift = 7;
+  static constexpr int kBytes = 2, kLift = 7, kLiftAgain = 7;
+  static constexpr uint32_t kInfinity = 0x7c00u;
   __device__ static f32x4 mma(const u32x4& a, const u32x4& b, const f32x4& c) { return ElemF16::mma(a, b, c, 0, 0); }
   __device__ static uint32_t pack(float lo, float hi) { return pack2_f16(lo, hi); }
   __device__ static float low(uint32_t w) { return f16_lo(w); }
@@ -80,9 +84,49 @@ struct F16 {
 };
 struct F32 {
   using Codec = CodecF32;
-  static constexpr int kBytes = 4, kLift = 0;
+  static constexpr int kBytes = 4, kLift = 0, kLiftAgain = kDown;
+  static constexpr uint32_t kInfinity = 0x7f800000u;
   __device__ static f32x4 mma(const u32x4& a, const u32x4& b, const f32x4& c) { return ElemF32::mma(a, b, c, 0, 0); }
 };
+
+// The infinite elements and those that are no numbers, zeros for the others.
+template <class T>
+__device__ inline u32x4 not_finite(u32x4 w) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (T::kBytes == 4) {
+      w[i] = (w[i] & T::kInfinity) == T::kInfinity ? w[i] : 0u;
+    } else {
+      const uint32_t low = (w[i] & T::kInfinity) == T::kInfinity ? w[i] & 0xffffu : 0u;
+      const uint32_t high = (w[i] >> 16 & T::kInfinity) == T::kInfinity ? w[i] & 0xffff0000u : 0u;
+      w[i] = low | high;
+    }
+  }
+  return w;
+}
+// Whether all are: 0 x is NaN if x is not. One comparison in the end, where one each took 0.3 us.
+template <int N>
+__device__ inline bool finite(const f32x4 (&v)[N]) {
+  f32x4 zero = v[0] * 0.0f;
+#pragma unroll
+  for (int f = 1; f < N; ++f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) zero[i] = __builtin_fmaf(v[f][i], 0.0f, zero[i]);
+  }
+  return (zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.0f;
+}
+__device__ inline bool finite(const f32x4& v) {
+  const f32x4 one[1] = {v};
+  return finite(one);
+}
+
+// A part's sums to those of all, by 2^kDown: where the sums of parts pass float32's range.
+__device__ inline void add_down(f32x4& o, float& total, const f32x4& part, const f32x2& stat, float base) {
+  const float p = __builtin_amdgcn_exp2f(stat[0] - base), down = __builtin_ldexpf(p, kDown);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] += (__builtin_fabsf(part[i]) < __builtin_inff() ? down : p) * part[i];
+  total += down * stat[1];
+}
 
 // How a chunk in memory becomes fragments of T: kFragments of 16 bytes.
 template <class T>
@@ -432,7 +476,16 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_attention(AttentionArgs a
   f32x4 out[kOut] = {};
   // P is taken by base: top - kLift, or 0 while there is none.
   float top = -__builtin_inff(), base = 0.0f, sum = 0.0f;
-  auto step = [&](const LdsPtr slot, uint32_t seen) __attribute__((always_inline)) {
+  // An infinite value makes NaN of what it should not where P has a low part (zero, or of the other sign) or is zero in
+  // 16 bits, and large ones of bfloat16 and float32 make an infinite sum of finite values. So where a wave has a sum
+  // that is not finite, it takes all its steps again, AGAIN, one at a time: infinite values count for themselves, by 1
+  // where their P is a normal float32, and P is scaled down. Codes of FP8 are not large. The look at the sums costs
+  // 0.1 us a call; all steps again as much as the call (64 sequences of up to 8192 positions, bf16: 201 us, with a NaN in
+  // every page 381).
+  constexpr int kLiftAgain = S::kBytes == 1 ? T::kLift : T::kLiftAgain;
+  auto step = [&](const LdsPtr slot, uint32_t seen, auto again) __attribute__((always_inline)) {
+    constexpr bool AGAIN = decltype(again)::value;
+    constexpr int kLift = AGAIN ? kLiftAgain : T::kLift;
     constexpr uint32_t kEvery = kStep == 32 ? 0xffffffffu : 0xffffu;
     const bool all = (seen & kEvery) == kEvery;
     u32x4 k[kTiles][kOfLane];
@@ -488,27 +541,30 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_attention(AttentionArgs a
       most = __builtin_fmaxf(most, __shfl_xor(most, 32));
       const float now = __builtin_fmaxf(top, most);
       const float keep = __builtin_amdgcn_exp2f(top - (now == -__builtin_inff() ? 0.0f : now));
-      base = now == -__builtin_inff() ? 0.0f : now - T::kLift;
+      base = now == -__builtin_inff() ? 0.0f : now - kLift;
       top = now;
       sum *= keep;
 #pragma unroll
       for (int f = 0; f < kOut; ++f) out[f] *= keep;
     }
+    f32x4 ones[kTiles];
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        if constexpr (AGAIN) ones[j][i] = score[j][i] - base + kLift >= -126.0f ? 1.0f : 0.0f;
         score[j][i] = __builtin_amdgcn_exp2f(score[j][i] - base);
         sum += score[j][i];
       }
     }
     // Elements past the head's are computed with what is in LDS there, and not stored.
     if constexpr (T::kBytes == 2) {
-      u32x4 high, low;
+      u32x4 high, low, one;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          if constexpr (AGAIN) one[2 * j + i] = T::pack(ones[j][2 * i], ones[j][2 * i + 1]);
           const float x = score[j][2 * i], y = score[j][2 * i + 1];
           const uint32_t h = T::pack(x, y);
           high[2 * j + i] = h;
@@ -534,10 +590,23 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_attention(AttentionArgs a
           S::four(x[1], e2);
           w = (u32x4){e[0], e[1], e2[0], e2[1]};
         }
+        if constexpr (AGAIN) {
+          const u32x4 rest = not_finite<T>(w);
+          out[f] = T::mma(rest, one, out[f]);
+          w ^= rest;
+        }
         out[f] = T::mma(w, high, out[f]);
         out[f] = T::mma(w, low, out[f]);
       }
     } else {
+      auto add = [&](f32x4& o, u32x4 w, int j) __attribute__((always_inline)) {
+        if constexpr (AGAIN) {
+          const u32x4 rest = not_finite<T>(w);
+          o = T::mma(rest, __builtin_bit_cast(u32x4, ones[j]), o);
+          w ^= rest;
+        }
+        o = T::mma(w, __builtin_bit_cast(u32x4, score[j]), o);
+      };
 #pragma unroll
       for (int f = 0; f < kOut; ++f) {
         if constexpr (S::kBytes == 4) {
@@ -547,14 +616,14 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_attention(AttentionArgs a
             const int r = 4 * g + i, c = (4 * f + (col >> 2)) ^ Sh::value_place(r);
             w[i] = lds_load<uint32_t>(from + r * kRow + c * 16 + (col & 3) * 4);
           }
-          out[f] = T::mma(w, __builtin_bit_cast(u32x4, score[0]), out[f]);
+          add(out[f], w, 0);
         } else {
           const u32x2 x = codes_at<Sh>(from, f, g, col);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             uint32_t e[4];
             S::four(x[j], e);
-            out[f] = T::mma((u32x4){e[0], e[1], e[2], e[3]}, __builtin_bit_cast(u32x4, score[j]), out[f]);
+            add(out[f], (u32x4){e[0], e[1], e[2], e[3]}, j);
           }
         }
       }
@@ -562,6 +631,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_attention(AttentionArgs a
   };
 
   const LdsPtr slots = (LdsPtr)lds;
+  int lift = T::kLift;
   if (WAVES == 1 || begin < end) {
     uint32_t seen[kDepth] = {};
     look(begin);
@@ -586,7 +656,7 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_attention(AttentionArgs a
           } else {
             loads_landed();
           }
-          step(slots + d * Sh::kSlot, seen[d]);
+          step(slots + d * Sh::kSlot, seen[d], std::false_type{});
           if (now + kDepth * kStep < end) {
             lds_read();
             seen[d] = ask(now + kDepth * kStep, slots + d * Sh::kSlot);
@@ -594,10 +664,24 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_attention(AttentionArgs a
         }
       }
     }
+    if (__builtin_expect(__any(!finite(out)), 0)) {
+      lift = kLiftAgain;
+      top = -__builtin_inff();
+      base = sum = 0.0f;
+#pragma unroll
+      for (int f = 0; f < kOut; ++f) out[f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      look(begin);
+      for (int first = begin; first < end; first += kStep) {
+        lds_read();
+        const uint32_t here = ask(first, slots);
+        loads_landed();
+        step(slots, here, std::true_type{});
+      }
+    }
   }
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
-  top -= T::kLift;  // the sums' power of two from here on
+  top -= lift;  // the sums' power of two from here on
 
   if constexpr (WAVES > 1) {
     // As join_parts, of the waves.
@@ -620,11 +704,21 @@ __global__ __launch_bounds__(64 * WAVES, 1) void paged_attention(AttentionArgs a
       }
       const float all_base = all_top == -__builtin_inff() ? 0.0f : all_top;
       f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+      auto part = [&](int w) __attribute__((always_inline)) {
+        return *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(rings[w]) + h * DIM + 4 * quad);
+      };
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
         const float p = __builtin_amdgcn_exp2f(stats[w][0] - all_base);
-        o += p * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(rings[w]) + h * DIM + 4 * quad);
+        o += p * part(w);
         total += p * stats[w][1];
+      }
+      if (__builtin_expect(S::kBytes > 1 && !finite(o), 0)) {
+        o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) add_down(o, total, part(w), stats[w], all_base);
+        all_top = all_base - kDown;
       }
       const int64_t head = (int64_t)sequence * a.heads + kv * group + head0 + h;
       const float inverse = total == 0.0f ? 0.0f : a.value_scale / total;
@@ -685,6 +779,7 @@ __global__ __launch_bounds__(THREADS) void join_parts(AttentionArgs a) {
   const int64_t stride = (int64_t)a.heads * a.dim;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   float top = -__builtin_inff(), total = 0.0f;
+  const bool large = a.value_scale == 1.0f;  // values may be: not those of an FP8 cache
   if (of < lanes) {
     for (int p0 = of; p0 < count; p0 += kAhead * lanes) {
       f32x4 part[kAhead];
@@ -709,6 +804,15 @@ __global__ __launch_bounds__(THREADS) void join_parts(AttentionArgs a) {
         total += w * stat[i][1];
       }
     }
+    if (__builtin_expect(large && !finite(o), 0)) {
+      const float base = top == -__builtin_inff() ? 0.0f : top;
+      o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      total = 0.0f;
+      for (int p = of; p < count; p += lanes) {
+        add_down(o, total, *reinterpret_cast<const f32x4*>(from + p * stride), stats[(int64_t)p * a.heads], base);
+      }
+      top = base - kDown;
+    }
   }
   sums[tid] = o;
   tops[tid] = (f32x2){top, total};
@@ -723,6 +827,12 @@ __global__ __launch_bounds__(THREADS) void join_parts(AttentionArgs a) {
     const float w = __builtin_amdgcn_exp2f(tops[i * quads + tid][0] - base);
     o += w * sums[i * quads + tid];
     total += w * tops[i * quads + tid][1];
+  }
+  if (__builtin_expect(large && !finite(o), 0)) {
+    o = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    total = 0.0f;
+    for (int i = 0; i < lanes; ++i) add_down(o, total, sums[i * quads + tid], tops[i * quads + tid], base);
+    all_top = base - kDown;
   }
   const float inverse = total == 0.0f ? 0.0f : a.value_scale / total;
   o = total == 0.0f ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : o * inverse;

@@ -57,7 +57,9 @@ def paged_attention(q: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
 
     Returns out ``[B, Hq, D]`` of q's dtype, and with ``return_lse`` the logarithm of each
     head's sum of exponentials, float32 ``[B, Hq]``, by which outputs over parts of a
-    context are joined. A sequence without positions: zeros, and -infinity."""
+    context are joined. A sequence without positions: zeros, and -infinity. An infinite
+    value that is seen makes its element infinite (NaN with one of the other sign, or where
+    its weight is less than float32 has); sequences that hold such, or NaN, take longer."""
     dim = q.shape[-1] if q.dim() else 0
     scale = float(dim or 1) ** -0.5 if scale is None else float(scale)
     # The ordinary call in one native call; None: the long way below, which raises the errors.
