@@ -665,6 +665,10 @@ inline bool rope_sizes_ok(const HeadsOf& q, const HeadsOf& k) {
 inline bool apart(const HeadsOf& h) {
   return ::apart(h.tokens, h.heads, h.dim, h.token_stride, h.head_stride);
 }
+// Where they lie: for tensors that are as the checks saw them.
+inline Region region(const Input& t, const HeadsOf& h) {
+  return {(uintptr_t)t.data(), dtype_bytes(float_tag(t)), h.tokens, h.heads, h.dim, h.token_stride, h.head_stride};
+}
 
 // (q, k, positions, frequencies, layout, scale, inverse, inplace); in place: True
 inline PyObject* rope_at(PyObject*, PyArgs a, Py_ssize_t n) {
@@ -691,7 +695,7 @@ inline PyObject* rope_at(PyObject*, PyArgs a, Py_ssize_t n) {
     allocate(q.device(), {{q.sizes(), q.type()}, {k.sizes(), k.type()}}, out);
   }
   if (!unchanged(q, k, positions, frequencies)) Py_RETURN_NONE;
-  if (inplace && q.data() == k.data()) Py_RETURN_NONE;
+  if (inplace && share(region(q, qh), region(k, kh))) Py_RETURN_NONE;
   check_launch("launch_rope_at_fwd",
                launch_rope_at_fwd(q.data(), k.data(), inplace ? q.data() : out[0].data_ptr(),
                                   inplace ? k.data() : out[1].data_ptr(), (const int64_t*)positions.data(),
@@ -740,6 +744,12 @@ inline PyObject* rope_to_cache(PyObject*, PyArgs a, Py_ssize_t n) {
                               inplace ? qh.head_stride : qh.dim};
   if (!inplace) allocate(q.device(), {{q.sizes(), q.type()}}, out);
   if (!unchanged(q, k, v, keys, values, slots, positions, frequencies)) Py_RETURN_NONE;
+  const int64_t cache_bytes = keys.numel() * (is_fp8(tag) ? 1 : dtype_bytes(tag));
+  const Region key_region((uintptr_t)keys.data(), cache_bytes), value_region((uintptr_t)values.data(), cache_bytes);
+  const Region heads[3] = {region(q, qh), region(k, kh), region(v, vh)};
+  bool shared = share(key_region, value_region) || (inplace && (share(heads[0], heads[1]) || share(heads[0], heads[2])));
+  for (const Region& h : heads) shared = shared || share(h, key_region) || share(h, value_region);
+  if (shared) Py_RETURN_NONE;
   check_launch("launch_rope_to_cache_fwd",
                launch_rope_to_cache_fwd(q.data(), k.data(), v.data(), inplace ? q.data() : out[0].data_ptr(),
                                         keys.data(), values.data(), (const int64_t*)slots.data(),

@@ -61,6 +61,69 @@ bool apart(int64_t tokens, int64_t heads, int64_t dim, int64_t token_stride, int
 }
 bool apart(const HeadsView& h) { return apart(h.tokens, h.heads, h.dim, h.token_stride, h.head_stride); }
 
+// Where heads lie, in bytes.
+struct Region {
+  int64_t at, tokens, heads, length, token_stride, head_stride;
+  Region(uintptr_t ptr, int64_t size, int64_t tokens, int64_t heads, int64_t dim, int64_t token_stride, int64_t head_stride)
+      : at((int64_t)ptr), tokens(tokens), heads(heads), length(dim * size), token_stride(tokens > 1 ? token_stride * size : 0),
+        head_stride(heads > 1 ? head_stride * size : 0) {}
+  // A contiguous tensor.
+  Region(uintptr_t ptr, int64_t bytes) : Region(ptr, 1, 1, 1, bytes, 0, 0) {}
+  bool empty() const { return tokens * heads * length == 0; }
+  int64_t extent() const { return (heads - 1) * head_stride + length; }  // of a token
+  int64_t end() const { return at + (tokens - 1) * token_stride + extent(); }
+};
+
+// Whether two tensors of heads have memory in common. Exact, but that those of one range with different strides
+// of their tokens, and with more than 2^20 pairs of heads at different strides, count as such.
+bool share(const Region& a, const Region& b) {
+  if (a.empty() || b.empty() || a.end() <= b.at || b.end() <= a.at) return false;
+  if (a.tokens > 1 && b.tokens > 1 && a.token_stride != b.token_stride) return true;
+  const int64_t period = a.tokens > 1 ? a.token_stride : b.token_stride, apart = b.at - a.at;
+  if (period > 0) {  // slices of a row side by side
+    const int64_t after = (apart % period + period) % period;
+    if (after >= a.extent() && after + b.extent() <= period) return false;
+  }
+  // x: from a head of a's to one of b's, of the same token; b's of another one are whole periods on.
+  const auto meet = [&](int64_t x) {
+    const auto by = [&](int64_t t) {
+      return t > -a.tokens && t < b.tokens && x + t * period < a.length && x + t * period > -b.length;
+    };
+    if (period <= 0) return by(0);
+    const int64_t t = std::clamp(-x / period, 1 - a.tokens, b.tokens - 1);
+    return by(t - 1) || by(t) || by(t + 1);
+  };
+  const bool even = a.heads == 1 || b.heads == 1 || a.head_stride == b.head_stride;
+  if (even) {
+    const int64_t stride = a.heads > 1 ? a.head_stride : b.head_stride;
+    for (int64_t d = 1 - a.heads; d < b.heads; ++d) {
+      if (meet(apart + d * stride)) return true;
+    }
+    return false;
+  }
+  if (a.heads > (int64_t(1) << 20) / b.heads) return true;
+  for (int64_t i = 0; i < a.heads; ++i) {
+    for (int64_t j = 0; j < b.heads; ++j) {
+      if (meet(apart + j * b.head_stride - i * a.head_stride)) return true;
+    }
+  }
+  return false;
+}
+Region region(const HeadsView& h) {
+  return {h.v.ptr, h.v.dtype == F32 ? 4 : 2, h.tokens, h.heads, h.dim, h.token_stride, h.head_stride};
+}
+Region region(const View& v) {
+  const int64_t size = v.dtype == F32 ? 4 : v.dtype == F16 || v.dtype == BF16 ? 2 : 1;
+  return {v.ptr, size * product(v.shape, 0, v.shape.size())};
+}
+// An output that is not the input itself.
+template <class A, class B>
+void check_apart(const char* out, const A& a, const char* other, const B& b) {
+  if (share(region(a), region(b))) {
+    value_error(std::string("arguments '") + out + "' and '" + other + "' are the same memory, or share some of it");
+  }
+}
+
 constexpr int64_t kMaxRopeDim = 2048;
 
 // Frequencies float64 [half] of heads of `dim`: half.
@@ -131,9 +194,11 @@ void rope_at_fwd(py::handle q, py::handle k, py::handle positions, py::handle fr
   check_rope_sizes(qv, kv);
   check_out("q_out", qo, qv, "q");
   check_out("k_out", ko, kv, "k");
-  if (qo.v.ptr == ko.v.ptr && qo.tokens * qo.heads * qo.dim > 0 && ko.heads > 0) {
-    value_error("arguments 'q_out' and 'k_out' are the same memory");
-  }
+  check_apart("q_out", qo, "k_out", ko);
+  check_apart("q_out", qo, "k", kv);
+  check_apart("k_out", ko, "q", qv);
+  if (qo.v.ptr != qv.v.ptr) check_apart("q_out", qo, "q", qv);
+  if (ko.v.ptr != kv.v.ptr) check_apart("k_out", ko, "k", kv);
   const int64_t strides[8] = {qv.token_stride, qv.head_stride, kv.token_stride, kv.head_stride,
                               qo.token_stride, qo.head_stride, ko.token_stride, ko.head_stride};
   const Launch launch(qv.v.device_index);
@@ -202,6 +267,18 @@ void rope_to_cache_fwd(py::handle q, py::handle k, py::handle v, py::handle key_
   const int64_t half = check_frequencies(fv, qv.dim, qv.v.device_index);
   check_rope_sizes(qv, kv);
   check_out("q_out", qo, qv, "q");
+  check_apart("q_out", qo, "k", kv);
+  check_apart("q_out", qo, "v", vv);
+  if (qo.v.ptr != qv.v.ptr) check_apart("q_out", qo, "q", qv);
+  check_apart("key_cache", kc, "value_cache", vc);
+  const auto check_cache_apart = [&](const char* name, const View& cache) {
+    check_apart(name, cache, "q_out", qo);
+    check_apart(name, cache, "q", qv);
+    check_apart(name, cache, "k", kv);
+    check_apart(name, cache, "v", vv);
+  };
+  check_cache_apart("key_cache", kc);
+  check_cache_apart("value_cache", vc);
   const int64_t strides[8] = {qv.token_stride, qv.head_stride, kv.token_stride, kv.head_stride,
                               vv.token_stride, vv.head_stride, qo.token_stride, qo.head_stride};
   const Launch launch(qv.v.device_index);

@@ -27,7 +27,8 @@ def rope_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_cache: 
 
     q ``[..., Hq, D]``, k and v ``[..., Hkv, D]``; ``slots``, ``positions``: int64 ``[...]``.
     A token whose slot is outside the cache (-1, say) is not written; no two tokens of a
-    call may have the same slot, which then would hold parts of both. Without frequencies
+    call may have the same slot, which then would hold parts of both. The caches share no
+    memory with each other or with q, k and v, nor q with k or v in place. Without frequencies
     (``[0]``) nothing turns. Into an FP8 cache go codes of the values divided by
     ``key_scale`` / ``value_scale``, those beyond the format's largest value as that."""
     # The ordinary call in one native call; None: the long way below, which raises the errors.

@@ -76,7 +76,7 @@ def rope_at(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, frequenci
     ``(x[2 i], x[2 i + 1])`` (``"interleaved"``). ``inverse`` turns by the negative angle:
     the gradient. q and k are contiguous, or ``[tokens, heads, D]`` with any strides of
     tokens and heads (slices of a projection's output). Returns contiguous tensors, or q
-    and k with ``inplace=True``."""
+    and k with ``inplace=True``, when they have no elements in common."""
     # The ordinary call in one native call; None: the long way below, which raises the errors.
     out = native.rope_at_call(q, k, positions, frequencies, layout, float(scale), inverse, inplace)
     if out is not None:

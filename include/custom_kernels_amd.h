@@ -272,7 +272,7 @@ int32_t launch_mxfp4_linear_fwd(const void* x_codes, const void* x_scales, const
  * the gradient. The other elements are copied. positions [tokens], frequencies float64
  * [half] (any position whose angle float64 holds). head_dim <= 2048. strides: token and
  * head strides of q, k, q_out, k_out (8 values). q_out == q and k_out == k (with their
- * strides) rotate in place. */
+ * strides) rotate in place; else outputs and inputs, and the two outputs, lie apart. */
 int32_t launch_rope_at_fwd(const void* q, const void* k, void* q_out, void* k_out, const int64_t* positions,
                            const void* frequencies, const int64_t* strides, int64_t tokens, int64_t n_q_heads,
                            int64_t n_kv_heads, int64_t head_dim, int64_t half, int32_t interleaved, int32_t inverse,
@@ -282,7 +282,8 @@ int32_t launch_rope_at_fwd(const void* q, const void* k, void* q_out, void* k_ou
  * n_kv_heads, head_dim] (slot = page * page_size + place in the page), of dtype
  * cache_dtype: dtype, or FP8 codes of the values divided by key_scale / value_scale
  * (within [1e-30, 1e30]), beyond the format's largest value to it. A token whose slot is
- * outside [0, cache_slots) is not written. Tokens of one call have slots of their own.
+ * outside [0, cache_slots) is not written. Tokens of one call have slots of their own,
+ * and the caches no memory in common with each other or with q, k, v and q_out.
  * strides: token and head strides of q, k, v, q_out (8 values). */
 int32_t launch_rope_to_cache_fwd(const void* q, const void* k, const void* v, void* q_out, void* key_cache,
                                  void* value_cache, const int64_t* slots, const int64_t* positions,
