@@ -778,7 +778,7 @@ inline PyObject* paged_attention(PyObject*, PyArgs a, Py_ssize_t n) {
   if (overflow != 0 || window < 0 || !qh || q.dim() != 3 || !keys || keys.dim() != 4 || !values || !table || !lengths) {
     Py_RETURN_NONE;
   }
-  const int64_t kv = keys.size(2), page = keys.size(1), width = table.size(-1);
+  const int64_t kv = keys.size(2), page = keys.size(1), width = table.dim() == 2 ? table.size(1) : 0;
   const int32_t tag = cache_tag(keys, q, kv);
   if (tag < 0 || tag != cache_tag(values, q, kv) || keys.sizes() != values.sizes() || !tokens_like(lengths, q) ||
       table.type() != c10::ScalarType::Long || table.device() != q.device() || table.dim() != 2 ||
