@@ -270,10 +270,16 @@ class LlamaBlock(nn.Module):
             raise ValueError(f"x must be [sequences, tokens, hidden] with the cache's {cache.lengths.shape[0]} sequences, "
                              f"got {tuple(x.shape)}")
 
-    def prefill(self, x: torch.Tensor, cache: PagedCache, positions: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+    def prefill(self, x: torch.Tensor, cache: PagedCache, positions: torch.Tensor, slots: torch.Tensor,
+                check: bool = True) -> torch.Tensor:
         """``forward`` of prompts ``[sequences, tokens, hidden]`` from position 0 on (of an empty cache), their keys
-        and values kept in ``cache``; positions and slots from its ``advance``."""
+        and values kept in ``cache``; positions and slots from its ``advance``, which makes all prompts equally long.
+        The prompt alone is attended to, so positions further on are refused. To tell, a call waits for the GPU, but not
+        while a graph is captured, nor with ``check=False``: of many layers the first one's check is enough."""
         self._check_serving(x, cache)
+        if check and not torch.cuda.is_current_stream_capturing() and bool(positions[..., :1].any()):
+            raise ValueError("prefill takes prompts from position 0 on, over an empty cache: what the cache holds would not "
+                             "be attended to")
         q, k, v, residual = self._project(x)
         rope_to_cache(q, k, v, cache.keys, cache.values, slots, positions, self.rope_frequencies,
                       key_scale=cache.key_scale, value_scale=cache.value_scale, inplace=True)
