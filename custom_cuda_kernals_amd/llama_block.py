@@ -103,7 +103,7 @@ class PagedCache:
         """An empty cache in which each sequence has all its pages."""
         each = -(-max_length // page_size)
         shape = (sequences * each, page_size, cfg.num_kv_heads, cfg.head_dim)
-        keys, values = (torch.zeros(shape, dtype=torch.float32, device=device).to(dtype) for _ in range(2))
+        keys, values = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
         table = torch.arange(sequences * each, device=device).view(sequences, each)
         return cls(keys, values, table, torch.zeros(sequences, dtype=torch.int64, device=device), key_scale, value_scale)
 
