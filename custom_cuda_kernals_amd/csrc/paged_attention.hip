@@ -959,7 +959,10 @@ extern "C" int64_t cck_paged_attention_workspace(int64_t sequences, int64_t n_q_
                                                  int32_t cache_dtype) {
   if (sequences <= 0 || !attention_sizes_ok(sequences, n_q_heads, n_kv_heads, head_dim, page_size, table_width)) return 0;
   const int64_t units = n_kv_heads * head_tiles_of(n_q_heads, n_kv_heads);
-  const int64_t parts = parts_of(sequences, units, page_size * table_width, head_dim, bytes_of(cache_dtype));
+  const int64_t positions = page_size * table_width, bytes = bytes_of(cache_dtype);
+  // With a window fewer positions are seen, which never makes parts of what is none without.
+  if (way_of(sequences * units, positions, head_dim, bytes) != kParts) return 0;
+  const int64_t parts = parts_of(sequences, units, positions, head_dim, bytes);
   return parts == 0 ? 0 : parts * n_q_heads * (head_dim + 2) * 4 + sequences * 8;
 }
 
