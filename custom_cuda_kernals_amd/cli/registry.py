@@ -490,7 +490,8 @@ REGISTRY: dict[str, OpSpec] = {
             target="within 2^-21 of the pair's size and one rounding of the float64 formula",
             reference=("an addition",), python_api=("rope_at", "rope_frequencies"),
             c_entry_points=("launch_rope_at_fwd",), sources=(_CSRC + "rotary.hip",),
-            test_files=("tests/test_rotary_gpu.py", "tests/test_decode_use_gpu.py", "tests/test_decode_cpu.py"),
+            test_files=("tests/test_rotary_gpu.py", "tests/test_shared_memory_gpu.py", "tests/test_decode_use_gpu.py",
+                        "tests/test_decode_cpu.py"),
             bench_ops=(), build_target=_t_rope_at),
         OpSpec(
             id="paged_attention", number=12, title="A paged key-value cache, and attention of one token over it",
@@ -506,8 +507,8 @@ REGISTRY: dict[str, OpSpec] = {
             reference=("an addition",), python_api=("rope_to_cache", "paged_attention"),
             c_entry_points=("launch_rope_to_cache_fwd", "launch_paged_attention_fwd"),
             sources=(_CSRC + "paged_attention.hip", _CSRC + "rotary.hip"),
-            test_files=("tests/test_paged_attention_gpu.py", "tests/test_rotary_gpu.py", "tests/test_decode_use_gpu.py",
-                        "tests/test_decode_cpu.py"),
+            test_files=("tests/test_paged_attention_gpu.py", "tests/test_paged_attention_values_gpu.py", "tests/test_rotary_gpu.py",
+                        "tests/test_prefill_gpu.py", "tests/test_decode_use_gpu.py", "tests/test_decode_cpu.py"),
             bench_ops=(), build_target=_t_paged_attention),
         OpSpec(
             id="fp8_linear", number=13, title="Products of FP8 with a scale for each block of 128",
@@ -518,11 +519,12 @@ REGISTRY: dict[str, OpSpec] = {
             design=("one matrix instruction a block of 128, its sums scaled into the tile's by the vector units",
                     "float32 results: exact products, as bfloat16",
                     "tiles and rings as grouped_linear's"),
-            target="block sums scaled in float32, one rounding; the same bits from every launch",
+            target="float32: sums of exact products; 16-bit: within 7 x 2^-13 of sum |x w|; the same bits from every launch",
             reference=("an addition",), python_api=("fp8_block_linear", "fp8_quant"),
             c_entry_points=("launch_fp8_block_linear_fwd", "launch_fp8_quant_group_fwd"),
             sources=(_CSRC + "fp8_linear.hip", _CSRC + "block_product.hpp", _CSRC + "tile_product.hpp"),
-            test_files=("tests/test_fp8_linear_gpu.py", "tests/test_decode_use_gpu.py", "tests/test_decode_cpu.py"),
+            test_files=("tests/test_fp8_linear_gpu.py", "tests/test_fp8_linear_exact_gpu.py", "tests/test_decode_use_gpu.py",
+                        "tests/test_decode_cpu.py"),
             bench_ops=(), build_target=_t_fp8_linear),
     ]
 }

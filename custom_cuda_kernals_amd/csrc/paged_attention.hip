@@ -24,8 +24,10 @@
 // while one is worked on, without registers or other waves to wait for.
 //
 // 8 key-value heads of 128: 64 sequences of up to 8192 positions, bf16, 1.08 GB, 192 us,
-// 5.6 TB/s (a copy reaches 5.2); two of 131072, e4m3, 0.54 GB, 106 us, 5.1 TB/s; 1024 of up
-// to 512 180 us, 5.9 TB/s; one of 700 10.4 us, where steps are waited for.
+// 5.6 TB/s (a copy of 1 GiB reaches 5.2, one of 320 MiB 6.7); two of 131072, e4m3, 0.54 GB,
+// 111 us, 4.8 TB/s; 1024 of up to 512 181 us, 5.9 TB/s; one of 700 10.3 us, where steps are
+// waited for. Worst: many short sequences in wide tables, as all parts read all lengths
+// (2048 of up to 100 positions 539 us in tables for 8192, 108 in tables for 112).
 #include "tile_product.hpp"
 
 namespace cck {
@@ -857,7 +859,7 @@ int64_t step_bytes(int64_t dim, int64_t cache_bytes) {
 // host takes half of the positions that the table has room for, the workgroups what there are: then many of the grid's
 // find nothing to do, so it is limited. bf16, 8 heads of 128, ragged, us, this and 8 parts a sequence: 64 of up to 8192
 // 191, 193; 128 of up to 4096 192, 205; 32 of up to 4096 55, 57; 64 of up to 1000 in tables for 131072 32, 36; 128 in
-// tables for 32768 57, 67; 64 of up to 32768 729, 712.
+// tables for 32768 57, 67. It loses with 64 of up to 32768: 729, 712.
 constexpr double kPartCost = 150;
 // Workgroups of a key-value head that fit the card.
 int64_t places_of(int64_t units, int64_t dim, int64_t cache_bytes) {

@@ -30,7 +30,8 @@ __device__ inline void lds_written() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_b
 
 // sin and cos of position * frequency. In quarter turns the whole part picks the quadrant
 // and the rest, at most half a quarter turn, is exact in float64; its float32 rounding is
-// 2^-25 of a radian. The series of Taylor to x^9 and x^10 end below 2e-9 at pi / 4.
+// 2^-25 of a radian. The series of Taylor to x^9 and x^10 end below 2e-9 at pi / 4. Three float64
+// roundings of the angle come before: 2^-51 of it together, which is less than the rest up to 2^28.
 __device__ inline f32x2 sin_cos(double position, double frequency) {
   const double quarters = position * (frequency * 0.63661977236758134308);  // 2 / pi
   const double whole = __builtin_rint(quarters);

@@ -24,14 +24,20 @@ __all__ = ["fp8_block_linear"]
 
 def fp8_block_linear(x_codes: torch.Tensor, x_scale: torch.Tensor, w_codes: torch.Tensor, w_scale: torch.Tensor,
                      offsets: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """``y = dequant(x) @ dequant(w).T``, sums in float32.
+    """``y = dequant(x) @ dequant(w).T``.
 
     x: codes ``[S, K]`` (``float8_e4m3fn`` or ``float8_e5m2``, w's the same or the other)
     with scales ``[S, ceil(K / 128)]`` (``"group"``) or ``[ceil(S / 128), ceil(K / 128)]``
     (``"block"``). w: ``[N, K]`` with ``[ceil(N / 128), ceil(K / 128)]``; with offsets
     (int64 ``[E + 1]``, as for ``grouped_linear``) ``[E, N, K]`` with ``[E, ceil(N / 128),
     ceil(K / 128)]``, and row ``s`` of expert ``e`` meets ``w[e]``, rows of no expert being
-    zeros. Returns y ``[S, N]`` of ``out_dtype`` (float32 / float16 / bfloat16)."""
+    zeros. Returns y ``[S, N]`` of ``out_dtype`` (float32 / float16 / bfloat16).
+
+    ``out_dtype`` chooses the sums. float32: of exact products, in float32. 16 bits: by the
+    FP8 matrix instructions, which cut off what is below 2^-13 of the largest of eight
+    neighbouring products, and in float32 beyond those eight. That is off by at most
+    ``7 * 2^-13 * sum |x w|`` and usually by 1e-5 of that sum, which is not small beside a
+    result whose products cancel. Where that matters, take float32 and round it."""
     # The ordinary call in one native call; None: the long way below, which raises the errors.
     out = native.fp8_block_linear_call(x_codes, x_scale, w_codes, w_scale, offsets, out_dtype)
     if out is not None:

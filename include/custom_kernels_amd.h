@@ -324,8 +324,11 @@ int32_t launch_fp8_quant_group_fwd(const void* x, uint8_t* x_fp8, float* scale, 
 /* y[s][j] = sum over k of x[s][k] w[e][j][k], y [rows, n] of dtype, of FP8 codes x [rows,
  * k] and w [num_experts, n, k] times their scales: x_scale [ceil(rows / x_block_rows),
  * ceil(k / 128)] with x_block_rows 1 or 128, w_scale [num_experts, ceil(n / 128), ceil(k /
- * 128)]. Sums in float32, each block's times its scales. offsets as for the expert
- * products, or NULL with num_experts == 1 for a dense product. Formats CCK_DTYPE_F8*. */
+ * 128)]. Each block's sum times its scales, in float32. offsets as for the expert
+ * products, or NULL with num_experts == 1 for a dense product. Formats CCK_DTYPE_F8*. A
+ * float32 result sums exact products in float32 (and so does any of k < 16); for a 16-bit
+ * one the FP8 matrix instructions cut off what is below 2^-13 of the largest of eight
+ * neighbouring products: 7 * 2^-13 * sum |x w| at most, usually 1e-5 of that sum. */
 int32_t launch_fp8_block_linear_fwd(const void* x, const float* x_scale, const void* w, const float* w_scale,
                                     const int64_t* offsets, void* y, int64_t rows, int64_t num_experts, int64_t n,
                                     int64_t k, int32_t x_block_rows, int32_t x_format, int32_t w_format, int32_t dtype,
