@@ -302,7 +302,7 @@ int32_t launch_rope_to_cache_fwd(const void* q, const void* k, const void* v, vo
  * 0, the last `window` of them; positions on a page outside [0, pages) are left out.
  * Where none is left, out is zeros and lse -infinity. lse [sequences, n_q_heads]: log of
  * the sum of the exponentials, or NULL. head_dim: a multiple of 16, at most 256.
- * workspace: cck_paged_attention_workspace(...) bytes, aligned to 16, for this call alone
+ * workspace: cck_paged_attention_workspace(...) bytes (0: NULL), aligned to 16, for this call alone
  * until it has run. */
 int32_t launch_paged_attention_fwd(const void* q, const void* key_cache, const void* value_cache,
                                    const int64_t* page_table, const int64_t* lengths, void* out, float* lse,
